@@ -423,6 +423,59 @@ int rcv_fcn_get_profile(rcv_fcn *h, double *conv_ms, double *other_ms, double *c
 /* Per-op device times (ms) of the last profiled forward; ms_out has room for n_ops doubles. */
 int rcv_fcn_get_op_times(rcv_fcn *h, double *ms_out, int n_ops);
 
+/* ------------------------------------------------------------------------------------------
+ * 8-bit integer products (no reference counterpart: the reference's forward is fp32, models/fcnresnet.py:121-191; an FCN engine
+ * in a 16-bit storage type runs chosen convolutions this way, rcv_op::wq_off)
+ * ------------------------------------------------------------------------------------------
+ * A token is one row of a channels-last tensor (a pixel of an NHWC activation).  It carries int8 codes and ONE float32 scale: the
+ * value of channel c is codes[c] * scale.  An output channel's weights likewise: int8 codes and one float32 scale.
+ *
+ * rcv_i8_quantize_tokens: x [rows, c0 + c1] -> codes, scales.  The channels come from one or two tensors of the same type (RCV_F32 /
+ * RCV_BF16 / RCV_F16), rows pitch0 / pitch1 elements apart (x1_dev NULL and c1 = 0: one).  scale = f32(max |x| / 127), code =
+ * round-half-even of the exact quotient x / scale, so codes are -127 .. 127.  A row whose scale falls below 2^-126, the all-zero row
+ * among them, gets scale 0 and codes 0; a row with a NaN or an infinity gets scale NaN and codes 0, which makes every
+ * product with it NaN.  Bytes between a row's last code and its pitch are left alone.
+ */
+int rcv_i8_quantize_tokens(const void *x0_dev, long long pitch0, int c0, const void *x1_dev, long long pitch1, int c1, int dtype,
+                           long long rows, int8_t *codes_dev, long long codes_pitch, float *scales_dev, void *stream);
+
+/*
+ * out[m, n] = act( sw[n] * sum_tap sa[m(tap)] * (sum_k codes[m(tap), k] * weights[n, tap, k]) + bias[n] + residual[m, n] )
+ *
+ * rcv_i8_matmul: one tap, m(tap) = m.  rcv_i8_conv3x3: the nine taps of a 3x3 window with zero padding and stride 1 over images of
+ * height x width tokens (rows = images * height * width, row-major).  Sums within a tap are exact 32-bit integers, taps are added
+ * in float32 in a fixed order, the result is rounded once to out_dtype: two calls give the same bits.  ReLU keeps a NaN.
+ *   codes       rows codes_pitch bytes apart; 16-byte aligned, codes_pitch a multiple of 16, and the last row readable up to
+ *               channels rounded up to a multiple of 16 (what lies there has no influence); -128 is allowed
+ *   weights     [out_channels][taps][channels rounded up to a multiple of 128], 16-byte aligned, zeros behind `channels`
+ *   bias        [out_channels] or NULL; residual [rows, residual_pitch] of out_dtype or NULL (may be `out` itself)
+ *   ws          device scratch of rcv_i8_*_workspace_bytes (0 where every call of that size runs without)
+ * channels <= 131071 (no sum can overflow), else RCV_E_TOO_LARGE.  rows = 0 does nothing.
+ */
+typedef struct rcv_i8_args {
+    uint32_t struct_bytes;     /* sizeof(rcv_i8_args) of the caller's header: RCV_E_INVALID when it is another's */
+    int32_t out_dtype;         /* RCV_F32 / RCV_BF16 / RCV_F16, of out and residual */
+    const int8_t *codes_dev;
+    const float *code_scales_dev;   /* [rows] */
+    const int8_t *weights_dev;
+    const float *weight_scales_dev; /* [out_channels] */
+    const float *bias_dev;
+    const void *residual_dev;
+    void *out_dev;
+    int64_t rows;
+    int64_t codes_pitch;       /* bytes */
+    int64_t residual_pitch;    /* elements */
+    int64_t out_pitch;         /* elements */
+    int32_t channels, out_channels;
+    int32_t height, width;     /* rcv_i8_conv3x3 */
+    int32_t relu;
+    int32_t reserved;
+} rcv_i8_args;
+size_t rcv_i8_matmul_workspace_bytes(long long rows, int channels, int out_channels);
+size_t rcv_i8_conv3x3_workspace_bytes(long long rows, int channels, int out_channels);
+int rcv_i8_matmul(const rcv_i8_args *args, void *ws, size_t ws_bytes, void *stream);
+int rcv_i8_conv3x3(const rcv_i8_args *args, void *ws, size_t ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -62,6 +62,15 @@ class AccResult(ctypes.Structure):
     ]
 
 
+class I8Args(ctypes.Structure):
+    """struct rcv_i8_args (include/rcvpose_hip.h)."""
+    _fields_ = [("struct_bytes", ctypes.c_uint32), ("out_dtype", ctypes.c_int32), ("codes", ctypes.c_void_p), ("code_scales", ctypes.c_void_p),
+                ("weights", ctypes.c_void_p), ("weight_scales", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p),
+                ("out", ctypes.c_void_p), ("rows", ctypes.c_int64), ("codes_pitch", ctypes.c_int64), ("residual_pitch", ctypes.c_int64),
+                ("out_pitch", ctypes.c_int64), ("channels", ctypes.c_int32), ("out_channels", ctypes.c_int32), ("height", ctypes.c_int32),
+                ("width", ctypes.c_int32), ("relu", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
 class Op(ctypes.Structure):
     _fields_ = [
         ("kind", ctypes.c_int32),
@@ -125,6 +134,11 @@ SYMBOLS = {
     "rcv_union_depth": (_i, [_vp, _vp, ctypes.c_longlong, _vp, _i, _i, _f, _vp, _i, _i, _vp, _vp]),
     "rcv_nn_distance": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp]),
     "rcv_icp_workspace_bytes": (_sz, [_i]),
+    "rcv_i8_quantize_tokens": (_i, [_vp, ctypes.c_longlong, _i, _vp, ctypes.c_longlong, _i, _i, ctypes.c_longlong, _vp, ctypes.c_longlong, _vp, _vp]),
+    "rcv_i8_matmul_workspace_bytes": (_sz, [ctypes.c_longlong, _i, _i]),
+    "rcv_i8_conv3x3_workspace_bytes": (_sz, [ctypes.c_longlong, _i, _i]),
+    "rcv_i8_matmul": (_i, [ctypes.POINTER(I8Args), _vp, _sz, _vp]),
+    "rcv_i8_conv3x3": (_i, [ctypes.POINTER(I8Args), _vp, _sz, _vp]),
     "rcv_icp_point_to_point": (_i, [_vp, _i, _vp, _i, _d, ctypes.POINTER(_d), _d, _d, _i, _vp, _vp, _sz, _vp]),
 }
 

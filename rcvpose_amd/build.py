@@ -24,6 +24,7 @@ SOURCES = {
     "fcn_x3.hip": [],    # ... and as the split-precision engine (half hi / lo pairs, three MFMAs per product)
     "pose.hip": ["-ffp-contract=off"],
     "icp.hip": ["-ffp-contract=off"],
+    "int8.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"],  # (scalar fp32 operations only; the host pass warns that it does not know the feature)
 }
 COMMON = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-I" + os.path.join(ROOT, "include"), "-I" + CSRC,
           "-Wall", "-Wno-unused-function"]

@@ -1,0 +1,200 @@
+"""8-bit integer products with one scale per token and one per output channel (rcv_i8_* in include/rcvpose_hip.h).
+
+    weight = quantize_weight(w)                          # once: [N, K], or a 3x3 convolution's [N, 3, 3, C] (channels last)
+    codes, scales = quantize_tokens(x)                   # x [..., C], float32 / bfloat16 / float16
+    y = matmul(codes, scales, weight, bias, relu=True)   # [..., N]
+    y = conv3x3(codes, scales, weight, bias)             # codes [B, H, W, C] -> [B, H, W, N], zero padding, stride 1
+
+A token is one row of a channels-last tensor; its value is codes * scale.  FcnEngine(int8=...) runs chosen convolutions of the FCN on
+these kernels.  Inference only; there is no CPU fallback.  Results do not depend on the run: integer sums are exact and float sums
+have a fixed order.  The reference has no counterpart (its forward is fp32, models/fcnresnet.py:121-191).
+"""
+import ctypes
+
+import torch
+
+from . import _hip
+
+KP = 128  # weight rows are zero-padded to a multiple of this many codes per tap (include/rcvpose_hip.h)
+MAX_CHANNELS = 131071
+_DTYPES = {torch.float32: _hip.RCV_F32, torch.bfloat16: _hip.RCV_BF16, torch.float16: _hip.RCV_F16}
+
+
+class Int8Weight:
+    """Packed weights of one layer: `codes` int8 [N, taps, K padded to a multiple of 128], `scales` float32 [N].
+    taps is 1 (matmul) or 9 (conv3x3)."""
+
+    def __init__(self, codes, scales, channels):
+        self.codes, self.scales, self.channels = codes, scales, channels
+        self.out_channels, self.taps = int(codes.shape[0]), int(codes.shape[1])
+
+    def to(self, device):
+        return Int8Weight(self.codes.to(device), self.scales.to(device), self.channels)
+
+    def dequantize(self):
+        """float32 [N, K] or [N, 3, 3, C]: the values the codes stand for."""
+        v = self.codes[:, :, :self.channels].float() * self.scales.view(-1, 1, 1)
+        return v[:, 0] if self.taps == 1 else v.view(self.out_channels, 3, 3, self.channels)
+
+
+def pack_codes(codes, scales):
+    """Int8Weight from codes [N, K] or [N, 3, 3, C] (int8) and one scale per output channel (float32 [N]), on the codes' device."""
+    if codes.dtype != torch.int8 or codes.dim() not in (2, 4) or (codes.dim() == 4 and tuple(codes.shape[1:3]) != (3, 3)):
+        raise ValueError("weight codes must be int8 [N, K] or [N, 3, 3, C]")
+    if scales.dtype != torch.float32 or tuple(scales.shape) != (codes.shape[0],) or scales.device != codes.device:
+        raise ValueError("weight scales must be float32 [N] on the codes' device")
+    n, k = codes.shape[0], codes.shape[-1]
+    if n == 0 or k == 0 or k > MAX_CHANNELS:
+        raise ValueError("an int8 weight needs at least one row and 1 ... %d channels" % MAX_CHANNELS)
+    taps = 1 if codes.dim() == 2 else 9
+    packed = torch.zeros(n, taps, (k + KP - 1) // KP * KP, dtype=torch.int8, device=codes.device)
+    packed[:, :, :k] = codes.reshape(n, taps, k)
+    return Int8Weight(packed, scales.contiguous(), int(k))
+
+
+def quantize_weight(w):
+    """Float weights [N, K] or [N, 3, 3, C] -> Int8Weight: one scale per output channel, max |w| / 127, codes rounded half to even
+    (in float64, on w's device: done once per layer).  A channel of zeros gets scale 0; non-finite weights raise ValueError."""
+    if not w.is_floating_point() or w.dim() not in (2, 4):
+        raise ValueError("weights must be floating point [N, K] or [N, 3, 3, C]")
+    flat = w.reshape(w.shape[0], -1).double()
+    if flat.numel() and not bool(torch.isfinite(flat).all()):
+        raise ValueError("weights are not finite")
+    scales = (flat.abs().amax(dim=1) / 127).float() if flat.numel() else torch.zeros(w.shape[0], device=w.device)
+    scales = torch.where(scales < 2.0 ** -126, torch.zeros_like(scales), scales)
+    if not bool(torch.isfinite(scales).all()):
+        raise ValueError("weights are beyond float32's range")
+    safe = torch.where(scales > 0, scales, torch.ones_like(scales)).double()
+    codes = torch.where(scales[:, None] > 0, torch.round(flat / safe[:, None]), torch.zeros_like(flat))
+    return pack_codes(codes.clamp_(-127, 127).to(torch.int8).view(w.shape), scales)
+
+
+def _rows(t, what):
+    """A channels-last tensor as (tensor, number of rows, row pitch in elements); anything whose leading dimensions do not walk rows at
+    one pitch is copied."""
+    c = t.shape[-1]
+    if t.is_contiguous():
+        return t, t.numel() // c if c else 0, c
+    if c == 1 or t.stride(-1) == 1:
+        rows, pitch, uniform = 1, None, True
+        for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if size == 1:
+                continue
+            if pitch is None:
+                pitch = stride
+            elif stride != pitch * rows:
+                uniform = False
+            rows *= size
+        pitch = c if pitch is None else pitch
+        if uniform and pitch >= c:
+            return t, rows, pitch
+    t = t.contiguous()
+    return t, t.numel() // c, c
+
+
+def _device(*tensors):
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("rcvpose_amd runs on MI355X only: move the tensors to 'cuda' (no CPU fallback)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError("all tensors of a call must be on one device")
+    return dev
+
+
+def quantize_tokens(x, x1=None):
+    """x [..., C] (float32, bfloat16 or float16), optionally a second tensor [..., C1] of the same type whose channels follow (the
+    concatenation is not materialised) -> (codes int8 [..., C + C1], scales float32 [...]).
+
+    scale = float32(max |x| / 127) of the token, code = x / scale rounded half to even.  A token of zeros gets scale 0; a token with a
+    NaN or an infinity gets scale NaN and codes 0, so products with it are NaN.  The rows of `codes` start 16 bytes aligned, as
+    matmul and conv3x3 need them: for C not a multiple of 16 `codes` is a view of a wider buffer."""
+    L = _hip.lib()
+    if x.dtype not in _DTYPES or x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError("tokens must be float32, bfloat16 or float16 [..., C] with at least one channel")
+    if x1 is not None and (x1.dtype != x.dtype or x1.shape[:-1] != x.shape[:-1] or x1.shape[-1] == 0):
+        raise ValueError("the second source must have the first one's type and leading dimensions")
+    c0, c1 = x.shape[-1], 0 if x1 is None else x1.shape[-1]
+    if c0 + c1 > MAX_CHANNELS:
+        raise ValueError("a token has at most %d channels" % MAX_CHANNELS)
+    dev = _device(x, x1)
+    with torch.cuda.device(dev):
+        x, rows, pitch0 = _rows(x, "tokens")
+        pitch1 = 0
+        if x1 is not None:
+            x1, _, pitch1 = _rows(x1, "tokens")
+        lead = x.shape[:-1]
+        pitch = (c0 + c1 + 15) // 16 * 16
+        codes = torch.empty(lead + (pitch,), dtype=torch.int8, device=dev)
+        scales = torch.empty(lead, dtype=torch.float32, device=dev)
+        if rows:
+            _hip.check(L.rcv_i8_quantize_tokens(x.data_ptr(), pitch0, c0, _hip.ptr(x1), pitch1, c1, _DTYPES[x.dtype], rows,
+                                                codes.data_ptr(), pitch, scales.data_ptr(), _hip.current_stream()),
+                       "rcv_i8_quantize_tokens")
+    return codes if pitch == c0 + c1 else codes[..., :c0 + c1], scales
+
+
+def _product(name, codes, scales, weight, bias, residual, relu, dtype, image):
+    L = _hip.lib()
+    k, n, lead = weight.channels, weight.out_channels, tuple(codes.shape[:-1])
+    if codes.dtype != torch.int8 or codes.dim() < 1 or codes.shape[-1] != k:
+        raise ValueError("codes must be int8 [..., %d] for this weight" % k)
+    if scales.dtype != torch.float32 or tuple(scales.shape) != lead:
+        raise ValueError("scales must be float32 with one value per token")
+    if dtype not in _DTYPES:
+        raise ValueError("output type must be torch.float32, torch.bfloat16 or torch.float16")
+    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (n,)):
+        raise ValueError("bias must be float32 [%d]" % n)
+    if residual is not None and (residual.dtype != dtype or tuple(residual.shape) != lead + (n,)):
+        raise ValueError("residual must have the output's type and shape")
+    dev = _device(codes, scales, weight.codes, bias, residual)
+    with torch.cuda.device(dev):
+        codes, rows, pitch = _rows(codes, "codes")
+        if rows == 1:  # (one row has no pitch of its own)
+            pitch = (k + 15) // 16 * 16
+        need = (rows - 1) * pitch + (k + 15) // 16 * 16
+        if rows and (pitch % 16 or codes.data_ptr() % 16 or codes.untyped_storage().nbytes() - codes.storage_offset() < need):
+            raise ValueError("token rows must start 16 bytes aligned and be readable up to a multiple of 16 channels: "
+                             "take the codes as quantize_tokens lays them out")
+        out = torch.empty(lead + (n,), dtype=dtype, device=dev)
+        if rows == 0:
+            return out
+        scales = scales.contiguous()
+        res_pitch = 0
+        if residual is not None:
+            residual, _, res_pitch = _rows(residual, "residual")
+        if bias is not None:
+            bias = bias.contiguous()
+        a = _hip.I8Args(ctypes.sizeof(_hip.I8Args), _DTYPES[dtype], codes.data_ptr(), scales.data_ptr(), weight.codes.data_ptr(),
+                        weight.scales.data_ptr(), None if bias is None else bias.data_ptr(),
+                        None if residual is None else residual.data_ptr(), out.data_ptr(), rows, pitch, res_pitch, n, k, n,
+                        image[0], image[1], int(bool(relu)), 0)
+        nbytes = getattr(L, name + "_workspace_bytes")(rows, k, n)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        _hip.check(getattr(L, name)(ctypes.byref(a), _hip.ptr(ws), nbytes, _hip.current_stream()), name)
+    return out
+
+
+def matmul(codes, scales, weight, bias=None, residual=None, relu=False, dtype=torch.bfloat16):
+    """act( (codes @ weight.T) * scales * weight scales + bias + residual ) -> [..., N] of `dtype`.
+
+    codes int8 [..., K] and scales float32 [...] as quantize_tokens gives them, weight an Int8Weight of [N, K], bias float32 [N],
+    residual [..., N] of `dtype`.  The integer sums are exact; the result is rounded once, to `dtype`.  relu keeps a NaN."""
+    if weight.taps != 1:
+        raise ValueError("matmul takes a weight packed from [N, K]; a 3x3 weight belongs to conv3x3")
+    return _product("rcv_i8_matmul", codes, scales, weight, bias, residual, relu, dtype, (0, 0))
+
+
+def conv3x3(codes, scales, weight, bias=None, residual=None, relu=False, dtype=torch.bfloat16):
+    """3x3 convolution with zero padding and stride 1 over tokens that form images: codes int8 [B, H, W, C], scales float32
+    [B, H, W], weight an Int8Weight of [N, 3, 3, C] -> [B, H, W, N] of `dtype`.  Every input pixel enters under its own scale: integer
+    sums over the channels of one tap are exact, the nine taps are added in float32.  bias, residual, relu as in matmul."""
+    if weight.taps != 9:
+        raise ValueError("conv3x3 takes a weight packed from [N, 3, 3, C]")
+    if codes.dim() != 4:
+        raise ValueError("codes must be int8 [B, H, W, C]")
+    return _product("rcv_i8_conv3x3", codes, scales, weight, bias, residual, relu, dtype, (int(codes.shape[1]), int(codes.shape[2])))

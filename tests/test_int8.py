@@ -1,0 +1,122 @@
+"""8-bit integer operators, the parts that need no GPU: weight packing and the refusals of the entry points (rcv_i8_* in
+include/rcvpose_hip.h check their arguments before anything is enqueued, so the codes come back here as well)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from rcvpose_amd import _hip, int8
+
+FAKE = 1 << 20  # an aligned address that no refused call touches
+
+
+def _args(**kw):
+    a = _hip.I8Args(ctypes.sizeof(_hip.I8Args), _hip.RCV_BF16, FAKE, FAKE, FAKE, FAKE, None, None, FAKE, 12, 64, 0, 32, 64, 32, 3, 4, 0, 0)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def _call(name, a):
+    return getattr(_hip.load_library(), name)(ctypes.byref(a), None, 0, None)
+
+
+@pytest.mark.parametrize("name", ["rcv_i8_matmul", "rcv_i8_conv3x3"])
+@pytest.mark.parametrize("change, status", [
+    (dict(struct_bytes=0), _hip.RCV_E_INVALID),
+    (dict(out_dtype=_hip.RCV_F16X3), _hip.RCV_E_UNSUPPORTED),
+    (dict(out_dtype=17), _hip.RCV_E_UNSUPPORTED),
+    (dict(rows=-12), _hip.RCV_E_INVALID),
+    (dict(channels=0), _hip.RCV_E_INVALID),
+    (dict(out_channels=0), _hip.RCV_E_INVALID),
+    (dict(channels=131072, codes_pitch=131072), _hip.RCV_E_TOO_LARGE),
+    (dict(codes=None), _hip.RCV_E_INVALID),
+    (dict(code_scales=None), _hip.RCV_E_INVALID),
+    (dict(weights=None), _hip.RCV_E_INVALID),
+    (dict(weight_scales=None), _hip.RCV_E_INVALID),
+    (dict(out=None), _hip.RCV_E_INVALID),
+    (dict(codes=FAKE + 4), _hip.RCV_E_INVALID),
+    (dict(weights=FAKE + 8), _hip.RCV_E_INVALID),
+    (dict(out=FAKE + 1), _hip.RCV_E_INVALID),
+    (dict(codes_pitch=72), _hip.RCV_E_INVALID),
+    (dict(codes_pitch=48), _hip.RCV_E_INVALID),
+    (dict(out_pitch=31), _hip.RCV_E_INVALID),
+    (dict(residual=FAKE, residual_pitch=31), _hip.RCV_E_INVALID),
+    (dict(residual=FAKE + 1, residual_pitch=32), _hip.RCV_E_INVALID),
+    (dict(codes_pitch=1 << 23), _hip.RCV_E_TOO_LARGE),
+    (dict(out_pitch=1 << 25), _hip.RCV_E_TOO_LARGE),
+])
+def test_product_refuses(name, change, status):
+    assert _call(name, _args(**change)) == status
+
+
+def test_conv_refuses_rows_that_are_no_images():
+    assert _call("rcv_i8_conv3x3", _args(rows=13)) == _hip.RCV_E_INVALID
+    assert _call("rcv_i8_conv3x3", _args(height=0)) == _hip.RCV_E_INVALID
+    assert _call("rcv_i8_conv3x3", _args(width=-4)) == _hip.RCV_E_INVALID
+    assert _call("rcv_i8_conv3x3", _args(height=1, width=1 << 17, rows=1 << 17)) == _hip.RCV_E_TOO_LARGE
+
+
+def test_no_rows_is_no_work():
+    for name in ("rcv_i8_matmul", "rcv_i8_conv3x3"):
+        assert _call(name, _args(rows=0)) == _hip.RCV_OK
+        assert getattr(_hip.load_library(), name + "_workspace_bytes")(0, 64, 32) == 0
+    assert _hip.load_library().rcv_i8_quantize_tokens(FAKE, 64, 64, None, 0, 0, _hip.RCV_F32, 0, FAKE, 64, FAKE, None) == _hip.RCV_OK
+
+
+@pytest.mark.parametrize("bad, status", [
+    (dict(x0=None), _hip.RCV_E_INVALID), (dict(c0=0), _hip.RCV_E_INVALID), (dict(c1=-1), _hip.RCV_E_INVALID),
+    (dict(c1=8, x1=None), _hip.RCV_E_INVALID), (dict(rows=-1), _hip.RCV_E_INVALID), (dict(codes=None), _hip.RCV_E_INVALID),
+    (dict(scales=None), _hip.RCV_E_INVALID), (dict(dtype=_hip.RCV_F16X3), _hip.RCV_E_UNSUPPORTED), (dict(pitch0=63), _hip.RCV_E_INVALID),
+    (dict(c1=8, x1=FAKE, pitch1=7, codes_pitch=72), _hip.RCV_E_INVALID), (dict(codes_pitch=63), _hip.RCV_E_INVALID),
+    (dict(c0=131072, pitch0=131072, codes_pitch=131072), _hip.RCV_E_TOO_LARGE), (dict(x0=FAKE + 1), _hip.RCV_E_INVALID),
+])
+def test_quantize_refuses(bad, status):
+    a = dict(x0=FAKE, pitch0=64, c0=64, x1=None, pitch1=0, c1=0, dtype=_hip.RCV_BF16, rows=4, codes=FAKE, codes_pitch=64, scales=FAKE)
+    a.update(bad)
+    assert _hip.load_library().rcv_i8_quantize_tokens(*a.values(), None) == status
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (5, 128), (7, 129), (6, 3, 3, 20)])
+def test_weight_quantisation(shape):
+    rng = np.random.default_rng(3)
+    w = rng.standard_normal(shape).astype(np.float32) * np.exp(rng.standard_normal((shape[0],) + (1,) * (len(shape) - 1))).astype(np.float32)
+    w[0] = 0
+    q = int8.quantize_weight(torch.from_numpy(w))
+    taps = 1 if len(shape) == 2 else 9
+    assert tuple(q.codes.shape) == (shape[0], taps, -(-shape[-1] // 128) * 128) and q.channels == shape[-1]
+    assert int(q.codes[:, :, shape[-1]:].abs().sum()) == 0
+    s = (np.abs(w.reshape(shape[0], -1)).max(axis=1).astype(np.float64) / 127).astype(np.float32)
+    np.testing.assert_array_equal(q.scales.numpy(), s)
+    ref = np.round(w.reshape(shape[0], -1).astype(np.float64) / np.where(s > 0, s, 1)[:, None].astype(np.float64)).reshape(shape)
+    np.testing.assert_array_equal(q.codes[:, :, :shape[-1]].numpy().reshape(shape), ref.astype(np.int8))
+    # a code is at most half a step away (plus float32's rounding of code * scale)
+    lim = s.reshape((-1,) + (1,) * (len(shape) - 1)) * (0.5 + 127 * 2.0 ** -23)
+    assert (np.abs(q.dequantize().numpy() - w) <= lim).all()
+
+
+def test_weight_refusals():
+    with pytest.raises(ValueError):
+        int8.quantize_weight(torch.tensor([[1.0, float("nan")]]))
+    with pytest.raises(ValueError):
+        int8.quantize_weight(torch.ones(4, 2, 3, 3))  # channels first
+    with pytest.raises(ValueError):
+        int8.quantize_weight(torch.ones(4, 4, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        int8.pack_codes(torch.ones(4, 4), torch.ones(4))
+    with pytest.raises(ValueError):
+        int8.pack_codes(torch.ones(4, 4, dtype=torch.int8), torch.ones(3))
+    with pytest.raises(ValueError):
+        int8.pack_codes(torch.ones(0, 4, dtype=torch.int8), torch.ones(0))
+    with pytest.raises(ValueError):
+        int8.pack_codes(torch.ones(1, 131072, dtype=torch.int8), torch.ones(1))
+
+
+def test_no_cpu_fallback():
+    if torch.cuda.is_available():
+        pytest.skip("GPU present")
+    with pytest.raises(_hip.HipLibraryError):
+        int8.quantize_tokens(torch.ones(2, 4))
+    with pytest.raises(_hip.HipLibraryError):
+        int8.matmul(torch.ones(2, 4, dtype=torch.int8), torch.ones(2), int8.quantize_weight(torch.ones(3, 4)))
