@@ -9,6 +9,8 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 #include "int8.hpp"
 
@@ -61,73 +63,528 @@ __global__ __launch_bounds__(256) void k_i8_quantize(const T *x0, long long pitc
     if (lane == 0) scales[row] = s;
 }
 
-// v = sum * sw + bias + residual, ReLU that keeps a NaN, rounded once to the output's type
-template <typename T>
-__device__ __forceinline__ void i8_store(const I8Product &p, long long m, int n, float v, int g, float &vmax)
+// A view of memory for buffer loads: what lies beyond `bytes` reads as zeros.
+__device__ __forceinline__ i32x4 descriptor(const int8_t *base, long long bytes)
 {
-    v = fmaf(v, p.weight_scales[(long long)g * p.weight_scale_gs + n], p.bias ? p.bias[(long long)g * p.bias_gs + n] : 0.f);
-    if (p.residual) v += as_f32(((const T *)p.residual)[(long long)g * p.residual_gs + m * p.residual_pitch + n]);
-    if (p.relu) v = v < 0.f ? 0.f : v;
-    vmax = fmaxf(vmax, fabsf(v));
-    ((T *)p.out)[(long long)g * p.out_gs + m * p.out_pitch + n] = as_out<T>(v);
+    const unsigned long long b = (unsigned long long)base;
+    const long long n = bytes < 0 ? 0 : bytes > 0x7fffffffLL ? 0x7fffffffLL : bytes;
+    return i32x4{(int)(unsigned)b, (int)((unsigned)(b >> 32) & 0xffffu), (int)n, 0x00020000};
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t view(const int8_t *base, long long bytes)
+{
+    return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, bytes < 0 ? 0 : bytes > 0x7fffffffLL ? 0x7fffffff : (int)bytes, 0x00020000);
+}
+__device__ __forceinline__ i32x4 load16(__amdgpu_buffer_rsrc_t rsrc, int voff, int soff)
+{
+    return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, voff, soff, 0));
 }
 
-// 64 tokens x 64 channels per workgroup, four waves of 32 x 32, operands straight from memory.
-template <typename T, int TAPS>
-__global__ __launch_bounds__(256) void k_i8_simple(const I8Product p)
+// Four channels n .. n + 3 of token m: v = sum * sw + bias + residual, ReLU that keeps a NaN, rounded once to the output's type.
+// `v` holds the sums with the token scales applied.  Returns the largest magnitude stored.
+template <typename T> __device__ __forceinline__ float finish_quad(const I8Product &p, int g, long long m, int n, const float *v)
 {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int r16 = lane & 15, kq = lane >> 4;
-    const int g = blockIdx.z;
-    const long long m0 = (long long)blockIdx.x * 64 + (wave >> 1) * 32;
-    const int n0 = blockIdx.y * 64 + (wave & 1) * 32;
-    const int8_t *codes = p.codes + (long long)g * p.code_gs * p.code_pitch;
-    const float *cs = p.code_scales + (long long)g * p.code_gs;
-    const int8_t *w = p.weights + (long long)g * p.Cout * TAPS * p.kp;
-    f32x4 sum[2][2];
-    for (int i = 0; i < 2; i++)
-        for (int j = 0; j < 2; j++) sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int tap = 0; tap < TAPS; tap++) {
-        long long src[2];
-        for (int j = 0; j < 2; j++) {
-            const long long m = m0 + j * 16 + r16;
-            src[j] = m < p.rows ? m : -1;
-            if (TAPS == 9 && m < p.rows) {
-                const int x = (int)(m % p.W), y = (int)(m / p.W % p.H), dy = tap / 3 - 1, dx = tap % 3 - 1;
-                src[j] = y + dy >= 0 && y + dy < p.H && x + dx >= 0 && x + dx < p.W ? m + (long long)dy * p.W + dx : -1;
-            }
-        }
-        i32x4 acc[2][2];
-        for (int i = 0; i < 2; i++)
-            for (int j = 0; j < 2; j++) acc[i][j] = i32x4{0, 0, 0, 0};
-        for (int k0 = 0; k0 < p.K; k0 += 64) {
-            const int k = k0 + kq * 16;
-            i32x4 wf[2], tf[2];
-            for (int i = 0; i < 2; i++) {
-                const int n = n0 + i * 16 + r16;
-                wf[i] = n < p.Cout ? *(const i32x4 *)(w + ((long long)n * TAPS + tap) * p.kp + k) : i32x4{0, 0, 0, 0};
-            }
-            // (a chunk that starts below K may end behind it: inside the row's pitch, and against weights that are zero there)
-            for (int j = 0; j < 2; j++)
-                tf[j] = src[j] >= 0 && k < p.K ? *(const i32x4 *)(codes + src[j] * p.code_pitch + k) : i32x4{0, 0, 0, 0};
-            for (int i = 0; i < 2; i++)
-                for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[i], tf[j], acc[i][j], 0, 0, 0);
-        }
-        for (int j = 0; j < 2; j++) {
-            const float sa = src[j] >= 0 ? cs[src[j]] : 0.f;
-            for (int i = 0; i < 2; i++)
-                for (int e = 0; e < 4; e++) sum[i][j][e] = fmaf((float)acc[i][j][e], sa, sum[i][j][e]);
-        }
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const float *ws = p.weight_scales + (long long)g * p.weight_scale_gs + n, *bias = p.bias ? p.bias + (long long)g * p.bias_gs + n : nullptr;
+    const T *res = p.residual ? (const T *)p.residual + (long long)g * p.residual_gs + m * p.residual_pitch + n : nullptr;
+    T *out = (T *)p.out + (long long)g * p.out_gs + m * p.out_pitch + n;
+    const bool whole = p.vec && n + 3 < p.Cout;
+    T4 r = T4{}, o;
+    if (res) {
+        if (whole) r = *(const T4 *)res;
+        else
+            for (int e = 0; e < 4; e++) if (n + e < p.Cout) r[e] = res[e];
     }
     float vmax = 0.f;
-    for (int i = 0; i < 2; i++)
-        for (int j = 0; j < 2; j++)
-            for (int e = 0; e < 4; e++) {
-                const long long m = m0 + j * 16 + r16;
-                const int n = n0 + i * 16 + kq * 4 + e;
-                if (m < p.rows && n < p.Cout) i8_store<T>(p, m, n, sum[i][j][e], g, vmax);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const bool live = n + e < p.Cout;
+        float y = fmaf(v[e], live ? ws[e] : 0.f, live && bias ? bias[e] : 0.f);
+        if (res) y += as_f32(r[e]);
+        if (p.relu) y = y < 0.f ? 0.f : y;
+        if (live) vmax = fmaxf(vmax, fabsf(y));
+        o[e] = as_out<T>(y);
+    }
+    if (whole) *(T4 *)out = o;
+    else
+        for (int e = 0; e < 4; e++) if (n + e < p.Cout) out[e] = o[e];
+    return vmax;
+}
+template <typename T> __device__ __forceinline__ void report_range(const I8Product &p, float vmax)
+{
+    if (sizeof(T) == 2 && p.range && vmax > 65504.f) atomicOr(p.range, 2u);
+}
+
+// ---------------------------------------------------------------------------------------------
+// operands straight from memory: few output tiles
+// ---------------------------------------------------------------------------------------------
+
+// TT * 16 tokens x CT * 16 channels per workgroup.  Its NW waves -- and the workgroups of gridDim.y -- divide the sum among themselves:
+// every wave multiplies its own run of 64-channel steps with nothing shared, D steps of loads in flight, so a short call is a few
+// memory round trips long.  The waves' sums meet in LDS and are added in order; with gridDim.y > 1 they go to `partial`
+// [split][group][rows][quads] and k_i8_finish adds them in order.  Integer sums (TAPS = 1) are exact whatever the order.
+template <typename T, int TAPS, int TT, int CT, int NW, int D>
+__global__ __launch_bounds__(64 * NW, 2) void k_i8_direct(const I8Product p, int tiles_n, f32x4 *partial)
+{
+    constexpr int OOB = (int)0x80000000, TILE_N = CT * 16, ROW = TILE_N + 4;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kq = lane >> 4;
+    const int g = blockIdx.z, mt = blockIdx.x / tiles_n, nt = blockIdx.x - mt * tiles_n, n0 = nt * TILE_N;
+    const long long m0 = (long long)mt * (TT * 16);
+    const int left = (int)min((long long)(TT * 16), p.rows - m0);
+    const int8_t *codes = p.codes + (long long)g * p.code_gs * p.code_pitch;
+    const int8_t *codes_end = codes + (p.rows - 1) * p.code_pitch + ((p.K + 15) & ~15);
+    const float *cs = p.code_scales + (long long)g * p.code_gs;
+    const int wrow = TAPS * p.kp, W = p.W, H = p.H;
+    const int8_t *wts = p.weights + ((long long)g * p.Cout + n0) * wrow;
+    const long long wbytes = (long long)(p.Cout - n0) * wrow;
+
+    int toff[TT], woff[CT];
+    unsigned inside[TT];
+#pragma unroll
+    for (int j = 0; j < TT; j++) {
+        const int row = j * 16 + r16;
+        toff[j] = row < left ? (int)(row * p.code_pitch) + kq * 16 : OOB;
+        inside[j] = 0u;
+        if (TAPS == 9 && row < left) {
+            const long long m = m0 + row, l = m / W;
+            const int x = (int)(m - l * W), y = (int)(l % H);
+            const unsigned cols = (x > 0 ? 1u : 0u) | 2u | (x + 1 < W ? 4u : 0u);
+            inside[j] = (y > 0 ? cols : 0u) | cols << 3 | (y + 1 < H ? cols << 6 : 0u);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < CT; i++) woff[i] = (i * 16 + r16) * wrow + kq * 16;
+
+    const int ksteps = (p.K + 63) / 64, nk = TAPS * ksteps;
+    const int unit = blockIdx.y * NW + wave, units = gridDim.y * NW;
+    const int s0 = (int)((long long)nk * unit / units), s1 = (int)((long long)nk * (unit + 1) / units);
+    int tap = TAPS == 9 ? s0 / ksteps : 0, ks = s0 - tap * ksteps;  // of the step being loaded
+    auto tap_shift = [&](int t) { return TAPS == 9 ? (long long)(t / 3 - 1) * W + (t % 3 - 1) : 0LL; };
+    auto load = [&](i32x4 *tf, i32x4 *wf, int step) {
+        if (step >= s1) return;
+        const int8_t *a = codes + (m0 + tap_shift(tap)) * p.code_pitch, *w = wts + (long long)tap * p.kp;
+        const __amdgpu_buffer_rsrc_t ra = view(a, codes_end - a), rw = view(w, wbytes - (long long)tap * p.kp);
+#pragma unroll
+        for (int i = 0; i < CT; i++) wf[i] = load16(rw, woff[i], ks * 64);
+#pragma unroll
+        for (int j = 0; j < TT; j++) tf[j] = load16(ra, TAPS == 1 || (inside[j] >> tap) & 1u ? toff[j] : OOB, ks * 64);
+        if (++ks == ksteps) { ks = 0; tap++; }
+    };
+
+    i32x4 acc[CT][TT], tf[2][D][TT], wf[2][D][CT];
+    f32x4 sum[CT][TT];
+#pragma unroll
+    for (int i = 0; i < CT; i++)
+#pragma unroll
+        for (int j = 0; j < TT; j++) {
+            acc[i][j] = i32x4{0, 0, 0, 0};
+            sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    int m_tap = TAPS == 9 ? s0 / ksteps : 0, m_ks = s0 - m_tap * ksteps;  // of the step being multiplied
+    auto step_of = [&](const i32x4 *t, const i32x4 *w, int step) {
+        if (step >= s1) return;
+#pragma unroll
+        for (int i = 0; i < CT; i++)
+#pragma unroll
+            for (int j = 0; j < TT; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], t[j], acc[i][j], 0, 0, 0);
+        if (TAPS == 9 && (++m_ks == ksteps || step + 1 == s1)) {  // the tokens of the next tap have scales of their own
+#pragma unroll
+            for (int j = 0; j < TT; j++) {
+                const float sa = (inside[j] >> m_tap) & 1u ? cs[m0 + j * 16 + r16 + tap_shift(m_tap)] : 0.f;
+#pragma unroll
+                for (int i = 0; i < CT; i++) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sum[i][j][e] = fmaf((float)acc[i][j][e], sa, sum[i][j][e]);
+                    acc[i][j] = i32x4{0, 0, 0, 0};
+                }
             }
-    if (p.range && sizeof(T) == 2 && vmax > 65504.f) atomicOr(p.range, 2u);
+            m_ks = 0;
+            m_tap++;
+        }
+    };
+#pragma unroll
+    for (int d = 0; d < D; d++) load(tf[0][d], wf[0][d], s0 + d);
+    for (int s = s0; s < s1; s += 2 * D) {
+#pragma unroll
+        for (int f = 0; f < 2; f++) {
+#pragma unroll
+            for (int d = 0; d < D; d++) load(tf[1 - f][d], wf[1 - f][d], s + (f + 1) * D + d);
+#pragma unroll
+            for (int d = 0; d < D; d++) step_of(tf[f][d], wf[f][d], s + f * D + d);
+        }
+    }
+
+    // the waves' sums meet: [wave][token][channel]
+#pragma unroll
+    for (int i = 0; i < CT; i++)
+#pragma unroll
+        for (int j = 0; j < TT; j++) {
+            const int at = ((wave * TT + j) * 16 + r16) * ROW + i * 16 + kq * 4;
+            if constexpr (TAPS == 9) ((f32x4 *)smem)[at / 4] = sum[i][j];
+            else ((i32x4 *)smem)[at / 4] = acc[i][j];
+        }
+    __syncthreads();
+    float vmax = 0.f;
+    for (int q = tid; q < TT * 16 * CT * 4; q += 64 * NW) {
+        const int row = q / (CT * 4), n = n0 + (q - row * (CT * 4)) * 4;
+        if (row >= left || n >= p.Cout) continue;
+        const int at = row * (ROW / 4) + (q - row * (CT * 4));
+        f32x4 v;
+        if constexpr (TAPS == 9) {
+            v = ((const f32x4 *)smem)[at];
+#pragma unroll
+            for (int w = 1; w < NW; w++) {
+                const f32x4 o = ((const f32x4 *)smem)[at + w * TT * 16 * (ROW / 4)];
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] += o[e];
+            }
+        } else {
+            i32x4 t = ((const i32x4 *)smem)[at];
+#pragma unroll
+            for (int w = 1; w < NW; w++) t += ((const i32x4 *)smem)[at + w * TT * 16 * (ROW / 4)];
+            v = __builtin_bit_cast(f32x4, t);
+        }
+        if (partial) {
+            const long long quads = (p.Cout + 3) / 4;
+            partial[(((long long)blockIdx.y * p.groups + g) * p.rows + m0 + row) * quads + n / 4] = v;
+            continue;
+        }
+        if constexpr (TAPS == 1) {
+            const i32x4 t = __builtin_bit_cast(i32x4, v);
+            const float sa = cs[m0 + row];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = (float)t[e] * sa;
+        }
+        vmax = fmaxf(vmax, finish_quad<T>(p, g, m0 + row, n, (const float *)&v));
+    }
+    report_range<T>(p, vmax);
+}
+
+// Adds the partial sums of a divided product in order and finishes.
+template <typename T, int TAPS> __global__ __launch_bounds__(256) void k_i8_finish(const I8Product p, const f32x4 *partial, int splits)
+{
+    const int quads = (p.Cout + 3) / 4, g = blockIdx.z;
+    const long long q = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (q >= p.rows * quads) return;
+    const long long m = q / quads, stride = (long long)p.groups * p.rows * quads;
+    const f32x4 *at = partial + (long long)g * p.rows * quads + q;
+    f32x4 v = at[0];
+    if constexpr (TAPS == 9) {
+        for (int s = 1; s < splits; s++) {
+            const f32x4 o = at[s * stride];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] += o[e];
+        }
+    } else {
+        i32x4 t = __builtin_bit_cast(i32x4, v);
+        for (int s = 1; s < splits; s++) t += __builtin_bit_cast(i32x4, at[s * stride]);
+        const float sa = p.code_scales[(long long)g * p.code_gs + m];
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = (float)t[e] * sa;
+    }
+    report_range<T>(p, finish_quad<T>(p, g, m, (int)(q - m * quads) * 4, (const float *)&v));
+}
+
+// ---------------------------------------------------------------------------------------------
+// operands through LDS
+// ---------------------------------------------------------------------------------------------
+
+// One piece of an operand tile: 64 lanes x 16 bytes from `rsrc` + soff + voff to LDS bytes [lds + LDS_OFF, + 1024).  Lanes whose offset (soff
+// included) is not below the descriptor's size deliver zeros.  (Inline: the compiler would wait for every piece before the next LDS
+// read of any stage.  The instruction has no register result; the kernel counts the pieces itself.)
+template <int LDS_OFF> __device__ __forceinline__ void dma16(i32x4 rsrc, int soff, unsigned lds, int voff)
+{
+    asm volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc), "s"(soff),
+                 "n"(LDS_OFF)
+                 : "m0", "scc");
+}
+template <int N> __device__ __forceinline__ void wait_pieces()  // all but the newest N pieces of this wave have landed, and its LDS reads are done
+{
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+
+template <int I, int N, typename F> __device__ __forceinline__ void for_each(F &&f)  // f(I) ... f(N - 1), each a compile-time constant
+{
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        for_each<I + 1, N>(f);
+    }
+}
+
+template <int TAPS_, int WT_, int WC_, int TT_, int CT_, int KB_, int NST_> struct TileShape {
+    static constexpr int TAPS = TAPS_, WT = WT_, WC = WC_, TT = TT_, CT = CT_, KB = KB_, NST = NST_;
+    static constexpr int NW = WT * WC, BM = WT * TT * 16, BN = WC * CT * 16;
+    static constexpr int RPP = 1024 / KB;                         // rows of one piece
+    static constexpr int PA = BM / RPP / NW, PB = BN / RPP / NW;  // pieces of a wave per step
+    static constexpr int P = PA + PB, STAGE = (BM + BN) * KB;
+    static constexpr int LDS = NST * STAGE + (TAPS == 9 ? 9 * BM * 4 : 0);
+    static_assert(BM % (RPP * NW) == 0 && BN % (RPP * NW) == 0 && LDS <= 160 * 1024 && (KB == 64 || KB == 128), "tile plan");
+    static_assert(TAPS == 1 || KB == 128, "a tap is a whole number of fragment pairs");
+};
+
+// BM tokens x BN channels per workgroup, WT x WC waves of TT x CT 16 x 16 tiles.  The weights are the matrix instruction's first operand, so a
+// lane ends up with four consecutive channels of one token.  A ring of NST stages of KB codes per row, filled NST - 1 steps ahead; rows are
+// KB bytes and the 16-byte chunks of a row are permuted (chunk ^= row bits) on the way in, so that the sixteen rows of a fragment
+// read fall on all banks.  One barrier per step.
+template <typename T, typename S>
+__global__ __launch_bounds__(64 * S::NW, S::NW == 8 ? 2 : 1) void k_i8_tile(const I8Product p, int tiles_m, int tiles_n)
+{
+    constexpr int TAPS = S::TAPS, TT = S::TT, CT = S::CT, KB = S::KB, NST = S::NST, PA = S::PA, P = S::P, BM = S::BM, BN = S::BN;
+    constexpr int OOB = (int)0x80000000;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)smem;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wt = wave / S::WC, wc = wave % S::WC, r16 = lane & 15, kq = lane >> 4;
+
+    // Workgroups go round-robin over the 8 XCDs: give every XCD a contiguous run of tiles, and walk a run in bands of eight
+    // token tiles, so that the tiles in flight on an XCD share both operands in its L2.
+    int mt, nt;
+    {
+        const unsigned total = gridDim.x, id = blockIdx.x, q = total / 8, r = total % 8, xcd = id % 8;
+        const unsigned s = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + id / 8;
+        const unsigned band = 8u * tiles_n, bi = s / band, in = s - bi * band;
+        const unsigned rows = min(8u, (unsigned)tiles_m - bi * 8);
+        nt = __builtin_amdgcn_readfirstlane((int)(in / rows));
+        mt = __builtin_amdgcn_readfirstlane((int)(bi * 8 + in % rows));
+    }
+    const int g = blockIdx.z, n0 = nt * BN;
+    const long long m0 = (long long)mt * BM;
+    const int left = (int)min((long long)BM, p.rows - m0);
+    const int8_t *codes = p.codes + (long long)g * p.code_gs * p.code_pitch;
+    const int8_t *codes_end = codes + (p.rows - 1) * p.code_pitch + ((p.K + 15) & ~15);
+    const float *cs = p.code_scales + (long long)g * p.code_gs;
+    const int wrow = TAPS * p.kp;
+    const int8_t *wts = p.weights + ((long long)g * p.Cout + n0) * wrow;
+    const long long wbytes = (long long)(p.Cout - n0) * wrow;
+
+    // which of the nine taps of a token lie inside its image
+    const int W = p.W, H = p.H;
+    int x0 = 0, y0 = 0;
+    if constexpr (TAPS == 9) {
+        const long long l = m0 / W;
+        x0 = __builtin_amdgcn_readfirstlane((int)(m0 - l * W));
+        y0 = __builtin_amdgcn_readfirstlane((int)(l % H));
+    }
+    auto taps_inside = [&](int row) -> unsigned {
+        if (row >= left) return 0u;
+        const int t = x0 + row, l = t / W, x = t - l * W, y = (y0 + l) % H;
+        const unsigned cols = (x > 0 ? 1u : 0u) | 2u | (x + 1 < W ? 4u : 0u);
+        return (y > 0 ? cols : 0u) | cols << 3 | (y + 1 < H ? cols << 6 : 0u);
+    };
+    float *sa_tab = (float *)(smem + NST * S::STAGE);  // [9][BM]: the scale under which a token's tap enters, 0 outside the image
+    if constexpr (TAPS == 9) {
+        for (int row = tid; row < BM; row += 64 * S::NW) {
+            const unsigned ok = taps_inside(row);
+#pragma unroll
+            for (int t = 0; t < 9; t++)
+                sa_tab[t * BM + row] = (ok >> t) & 1u ? cs[m0 + row + (long long)(t / 3 - 1) * W + (t % 3 - 1)] : 0.f;
+        }
+    }
+
+    // this lane's part of the pieces: row lane / (KB / 16) of the piece, 16-byte slot lane % (KB / 16)
+    constexpr int LPR = KB / 16;
+    auto chunk_of = [&](int row, int slot) { return KB == 128 ? slot ^ ((row >> 1) & 7) : slot ^ (-(row >> 2) & 3); };
+    int voff[P];
+    unsigned inside[TAPS == 9 ? PA : 1];
+#pragma unroll
+    for (int c = 0; c < P; c++) {
+        const bool tok = c < PA;
+        const int row = (tok ? wave * PA + c : wave * S::PB + c - PA) * S::RPP + lane / LPR;
+        const int chunk = chunk_of(row, lane % LPR) * 16;
+        if (tok) {
+            voff[c] = row < left ? (int)(row * p.code_pitch) + chunk : OOB;
+            if constexpr (TAPS == 9) inside[c] = taps_inside(row);
+        } else
+            voff[c] = row * wrow + chunk;
+    }
+
+    // The step being issued.  Behind the last step the pieces go on with every lane out of range (`done`), which keeps the counts the same.
+    const int ksteps = KB == 64 ? p.kp / KB : (p.K + KB - 1) / KB, nk = TAPS * ksteps;  // (pairs of steps: the weights are zero up to kp)
+    const long long pitch = p.code_pitch;
+    int i_tap = 0, i_k = 0, i_left = nk, done = 0;
+    unsigned i_lds = lds0 + wave * PA * 1024;
+    const unsigned lds_w = BM * KB + (wave * S::PB - wave * PA) * 1024, lds_end = i_lds + NST * S::STAGE;
+    i32x4 ra, rw;
+    auto begin_tap = [&]() {
+        const int8_t *a = codes + (m0 + (TAPS == 9 ? (long long)(i_tap / 3 - 1) * W + (i_tap % 3 - 1) : 0)) * pitch;
+        ra = descriptor(a, codes_end - a);
+        rw = descriptor(wts + (long long)i_tap * p.kp, wbytes - (long long)i_tap * p.kp);
+    };
+    auto piece = [&](auto cc) {
+        constexpr int c = decltype(cc)::value;
+        if constexpr (c < PA) {
+            int v = voff[c];
+            if constexpr (TAPS == 9) v = (inside[c] >> i_tap) & 1u ? v : OOB;  // (no bit is set behind the ninth tap)
+            else v |= done;
+            dma16<c * 1024>(ra, i_k, i_lds, v);
+        } else
+            dma16<(c - PA) * 1024>(rw, i_k, i_lds + lds_w, voff[c] | done);
+    };
+    auto end_step = [&]() {
+        i_lds = i_lds + S::STAGE == lds_end ? lds_end - NST * S::STAGE : i_lds + S::STAGE;
+        i_left--;
+        done = i_left > 0 ? 0 : OOB;
+        i_k += KB;
+        if (TAPS == 9 && i_k == ksteps * KB) {
+            i_k = 0;
+            i_tap++;
+            if (i_tap < 9) begin_tap();
+        }
+    };
+
+    begin_tap();
+    asm volatile("s_nop 4");  // (scalars that came through vector registers, before the first piece reads them)
+    for (int s = 0; s < NST; s++) {
+        for_each<0, P>(piece);
+        end_step();
+    }
+
+    i32x4 acc[CT][TT];
+    f32x4 sum[TAPS == 9 ? CT : 1][TAPS == 9 ? TT : 1];
+#pragma unroll
+    for (int i = 0; i < CT; i++)
+#pragma unroll
+        for (int j = 0; j < TT; j++) {
+            acc[i][j] = i32x4{0, 0, 0, 0};
+            if constexpr (TAPS == 9) sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    i32x4 tf[2][TT], wf[2][CT];
+    const int t_row = (wt * TT * 16 + r16) * KB, w_row = BM * KB + (wc * CT * 16 + r16) * KB;
+    int r_stage = 0;  // byte offset of the stage being read
+    auto read = [&](int f, int half, int q) {  // fragment q of set f
+        const int slot = chunk_of(r16, half * 4 + kq) * 16;
+        if (q < TT) tf[f][q] = *(const i32x4 *)(smem + r_stage + t_row + slot + q * 16 * KB);
+        else wf[f][q - TT] = *(const i32x4 *)(smem + r_stage + w_row + slot + (q - TT) * 16 * KB);
+    };
+    auto next_stage = [&]() { r_stage = r_stage + S::STAGE == NST * S::STAGE ? 0 : r_stage + S::STAGE; };
+    // all products of fragment set f; meanwhile the other set is read (from `half` of the current read stage) and pieces [lo, hi) are issued
+    constexpr int NM = TT * CT, NF = TT + CT, SEG = NM / 4;
+    auto multiply = [&](auto ff, int half, auto lo_, auto hi_) {
+        constexpr int f = decltype(ff)::value, lo = decltype(lo_)::value, hi = decltype(hi_)::value;
+        for_each<0, SEG>([&](auto ss) {
+            constexpr int s = decltype(ss)::value;
+#pragma unroll
+            for (int q = s * NF / SEG; q < (s + 1) * NF / SEG; q++) read(1 - f, half, q);
+            for_each<lo + s * (hi - lo) / SEG, lo + (s + 1) * (hi - lo) / SEG>(piece);
+#pragma unroll
+            for (int e = s * 4; e < s * 4 + 4; e++) {
+                const int i = e / TT, j = e % TT;
+                acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[f][i], tf[f][j], acc[i][j], 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    constexpr std::integral_constant<int, 0> c0{};
+    constexpr std::integral_constant<int, 1> c1{};
+    constexpr std::integral_constant<int, P / 2> ch{};
+    constexpr std::integral_constant<int, P> cp{};
+
+    wait_pieces<P *(NST - 1)>();
+    __builtin_amdgcn_s_barrier();
+#pragma unroll
+    for (int q = 0; q < NF; q++) read(0, 0, q);
+    if constexpr (KB == 128) {
+        // a step's pieces are spread over its second half and the next step's first
+        bool first = true;
+        for (int tap = 0; tap < TAPS; tap++) {
+            for (int ks = 0; ks < ksteps; ks++) {
+                if (first) multiply(c0, 1, cp, cp);
+                else {
+                    multiply(c0, 1, ch, cp);
+                    end_step();
+                }
+                first = false;
+                wait_pieces<P *(NST - 2)>();  // the next stage is here; nobody reads the current one any more
+                __builtin_amdgcn_s_barrier();
+                next_stage();
+                multiply(c1, 0, c0, ch);
+            }
+            if constexpr (TAPS == 9) {
+#pragma unroll
+                for (int j = 0; j < TT; j++) {
+                    const float sa = sa_tab[tap * BM + wt * TT * 16 + j * 16 + r16];
+#pragma unroll
+                    for (int i = 0; i < CT; i++) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) sum[i][j][e] = fmaf((float)acc[i][j][e], sa, sum[i][j][e]);
+                        acc[i][j] = i32x4{0, 0, 0, 0};
+                    }
+                }
+            }
+        }
+    } else {
+        for (int ks = 0; ks < nk; ks += 2) {
+            for_each<0, 2>([&](auto f) {
+                wait_pieces<P *(NST - 2)>();
+                __builtin_amdgcn_s_barrier();
+                next_stage();
+                multiply(f, 0, c0, cp);
+                end_step();
+            });
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // (the last pieces: zeros nobody reads)
+
+    // epilogue: four channels of a token at a time, straight from the registers
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    float vmax = 0.f;
+    T *out = (T *)p.out + (long long)g * p.out_gs;
+    const T *res = p.residual ? (const T *)p.residual + (long long)g * p.residual_gs : nullptr;
+    const float *bias = p.bias ? p.bias + (long long)g * p.bias_gs : nullptr, *ws = p.weight_scales + (long long)g * p.weight_scale_gs;
+    float sa[TT];
+#pragma unroll
+    for (int j = 0; j < TT; j++) {
+        const int row = wt * TT * 16 + j * 16 + r16;
+        sa[j] = TAPS == 1 && row < left ? cs[m0 + row] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < CT; i++) {
+        const int n = n0 + (wc * CT + i) * 16 + kq * 4;
+        float b4[4], s4[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            b4[e] = bias && n + e < p.Cout ? bias[n + e] : 0.f;
+            s4[e] = n + e < p.Cout ? ws[n + e] : 0.f;
+        }
+        const bool whole = p.vec && n + 3 < p.Cout;
+        T4 r4[TT];
+#pragma unroll
+        for (int j = 0; j < TT; j++) {
+            const int row = wt * TT * 16 + j * 16 + r16;
+            const long long at = (m0 + row) * p.residual_pitch + n;
+            r4[j] = T4{};
+            if (!res || row >= left) continue;
+            if (whole) r4[j] = *(const T4 *)(res + at);
+            else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) if (n + e < p.Cout) r4[j][e] = res[at + e];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < TT; j++) {
+            const int row = wt * TT * 16 + j * 16 + r16;
+            const long long at = (m0 + row) * p.out_pitch + n;
+            T4 o;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                float v;
+                if constexpr (TAPS == 9) v = sum[i][j][e];
+                else v = (float)acc[i][j][e] * sa[j];
+                v = fmaf(v, s4[e], b4[e]);
+                if (res) v += as_f32(r4[j][e]);
+                if (p.relu) v = v < 0.f ? 0.f : v;  // (a NaN stays)
+                if (row < left && n + e < p.Cout) vmax = fmaxf(vmax, fabsf(v));
+                o[e] = as_out<T>(v);
+            }
+            if (row >= left) continue;
+            if (whole) *(T4 *)(out + at) = o;
+            else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) if (n + e < p.Cout) out[at + e] = o[e];
+            }
+        }
+    }
+    report_range<T>(p, vmax);
 }
 
 template <typename T> int launch_quantize(const void *x0, long long pitch0, int c0, const void *x1, long long pitch1, int c1, long long rows,
@@ -139,13 +596,87 @@ template <typename T> int launch_quantize(const void *x0, long long pitch0, int 
     return RCV_OK;
 }
 
-template <typename T> int launch_product(const I8Product &p, void *, size_t, hipStream_t st)
+// Lets `kernel` use more than the default 64 KB of LDS on the current device, once (ready: one bit per device).
+int allow_lds(const void *kernel, int bytes, std::atomic<unsigned long long> &ready)
 {
-    const dim3 grid((unsigned)((p.rows + 63) / 64), (unsigned)((p.Cout + 63) / 64), p.groups);
-    if (p.taps == 1) hipLaunchKernelGGL((k_i8_simple<T, 1>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((k_i8_simple<T, 9>), grid, dim3(256), 0, st, p);
+    int dev = 0;
+    RCV_HIP_CHECK(hipGetDevice(&dev));
+    if (dev < 64 && ready.load(std::memory_order_acquire) >> dev & 1) return RCV_OK;
+    RCV_HIP_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (dev < 64) ready.fetch_or(1ULL << dev, std::memory_order_release);
+    return RCV_OK;
+}
+
+template <typename T, typename S> int launch_tile(const I8Product &p, hipStream_t st)
+{
+    static std::atomic<unsigned long long> ready{0};
+    const int rc = allow_lds((const void *)k_i8_tile<T, S>, S::LDS, ready);
+    if (rc != RCV_OK) return rc;
+    const long long tm = (p.rows + S::BM - 1) / S::BM, tn = (p.Cout + S::BN - 1) / S::BN;
+    if (tm * tn > 0x7fffffffLL) return RCV_E_TOO_LARGE;
+    hipLaunchKernelGGL((k_i8_tile<T, S>), dim3((unsigned)(tm * tn), 1, p.groups), dim3(64 * S::NW), S::LDS, st, p, (int)tm, (int)tn);
     RCV_LAUNCH_CHECK();
     return RCV_OK;
+}
+
+// How a product runs.
+struct Plan {
+    enum Kind { TILE, DIRECT64, DIRECT16 } kind;
+    int splits;
+    size_t bytes;  // of partial sums
+};
+
+Plan plan_product(long long rows, int K, int Cout, int taps, int groups)
+{
+    Plan pl{Plan::TILE, 1, 0};
+    const long long tiles = ((rows + 255) / 256) * ((Cout + 127) / 128) * groups;
+    if (tiles >= 128) return pl;
+    pl.kind = rows <= 16 ? Plan::DIRECT16 : Plan::DIRECT64;
+    const int edge = rows <= 16 ? 16 : 64;
+    const long long wgs = ((rows + edge - 1) / edge) * ((Cout + edge - 1) / edge) * groups;
+    const int steps = taps * ((K + 63) / 64);
+    while (wgs * pl.splits * 2 <= 512 && steps >= pl.splits * 2 * 8 * 4) pl.splits *= 2;  // (at least four steps a wave)
+    if (pl.splits > 1) pl.bytes = (size_t)pl.splits * groups * rows * ((Cout + 3) / 4) * 16;
+    return pl;
+}
+
+template <typename T, int TAPS, int TT, int CT> int launch_direct(const I8Product &p, const Plan &pl, void *ws, hipStream_t st)
+{
+    constexpr int NW = 8, D = TT == 1 ? 4 : 1, LDS = NW * TT * 16 * (CT * 16 + 4) * 4;
+    static std::atomic<unsigned long long> ready{0};
+    if (LDS > 64 * 1024) {
+        const int rc = allow_lds((const void *)k_i8_direct<T, TAPS, TT, CT, NW, D>, LDS, ready);
+        if (rc != RCV_OK) return rc;
+    }
+    const long long tm = (p.rows + TT * 16 - 1) / (TT * 16), tn = (p.Cout + CT * 16 - 1) / (CT * 16);
+    if (tm * tn > 0x7fffffffLL) return RCV_E_TOO_LARGE;
+    f32x4 *partial = pl.splits > 1 ? (f32x4 *)ws : nullptr;
+    hipLaunchKernelGGL((k_i8_direct<T, TAPS, TT, CT, NW, D>), dim3((unsigned)(tm * tn), pl.splits, p.groups), dim3(64 * NW), LDS, st, p, (int)tn,
+                       partial);
+    RCV_LAUNCH_CHECK();
+    if (partial) {
+        const long long quads = p.rows * ((p.Cout + 3) / 4);
+        hipLaunchKernelGGL((k_i8_finish<T, TAPS>), dim3((unsigned)((quads + 255) / 256), 1, p.groups), dim3(256), 0, st, p,
+                           (const f32x4 *)partial, pl.splits);
+        RCV_LAUNCH_CHECK();
+    }
+    return RCV_OK;
+}
+
+template <typename T, int TAPS> int launch_taps(const I8Product &p, const Plan &pl, void *ws, hipStream_t st)
+{
+    if (pl.kind == Plan::TILE) return launch_tile<T, TileShape<TAPS, 4, 2, 4, 4, 128, 3>>(p, st);
+    if (pl.kind == Plan::DIRECT16) return launch_direct<T, TAPS, 1, 1>(p, pl, ws, st);
+    return launch_direct<T, TAPS, 4, 4>(p, pl, ws, st);
+}
+
+template <typename T> int launch_product(I8Product p, void *ws, hipStream_t st)
+{
+    const size_t four = 4 * sizeof(T);  // rows of output (and residual) that can be moved four channels at a time
+    p.vec = (uintptr_t)p.out % four == 0 && p.out_pitch % 4 == 0 && p.out_gs % 4 == 0 &&
+            (!p.residual || ((uintptr_t)p.residual % four == 0 && p.residual_pitch % 4 == 0 && p.residual_gs % 4 == 0));
+    const Plan pl = plan_product(p.rows, p.K, p.Cout, p.taps, p.groups);
+    return p.taps == 9 ? launch_taps<T, 9>(p, pl, ws, st) : launch_taps<T, 1>(p, pl, ws, st);
 }
 
 }  // namespace
@@ -159,15 +690,20 @@ int i8_quantize(const void *x0, long long pitch0, int c0, const void *x1, long l
     return launch_quantize<_Float16>(x0, pitch0, c0, x1, pitch1, c1, rows, codes, codes_pitch, scales, st);
 }
 
-size_t i8_product_workspace(long long, int, int, int, int) { return 0; }
+size_t i8_product_workspace(long long rows, int K, int Cout, int taps, int groups)
+{
+    return rows > 0 ? plan_product(rows, K, Cout, taps, groups).bytes : 0;
+}
 
 int i8_product(const I8Product &p, void *ws, size_t ws_bytes, hipStream_t st)
 {
     if (p.rows == 0) return RCV_OK;
-    if (ws_bytes < i8_product_workspace(p.rows, p.K, p.Cout, p.taps, p.groups)) return RCV_E_WORKSPACE;
-    if (p.out_dtype == RCV_F32) return launch_product<float>(p, ws, ws_bytes, st);
-    if (p.out_dtype == RCV_BF16) return launch_product<__bf16>(p, ws, ws_bytes, st);
-    return launch_product<_Float16>(p, ws, ws_bytes, st);
+    const size_t need = i8_product_workspace(p.rows, p.K, p.Cout, p.taps, p.groups);
+    if (need && (ws_bytes < need || !ws)) return RCV_E_WORKSPACE;
+    if ((uintptr_t)ws % 16) return RCV_E_INVALID;
+    if (p.out_dtype == RCV_F32) return launch_product<float>(p, ws, st);
+    if (p.out_dtype == RCV_BF16) return launch_product<__bf16>(p, ws, st);
+    return launch_product<_Float16>(p, ws, st);
 }
 
 }  // namespace rcv
