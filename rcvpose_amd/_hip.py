@@ -219,3 +219,10 @@ def current_stream():
     import torch
 
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def raw_stream(index):
+    """hipStream_t of device `index`'s current stream, as an integer (current_stream without the Stream object: 4 us less per call)."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(index)

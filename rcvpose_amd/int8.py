@@ -17,6 +17,7 @@ from . import _hip
 
 KP = 128  # weight rows are zero-padded to a multiple of this many codes per tap (include/rcvpose_hip.h)
 MAX_CHANNELS = 131071
+_ARGS_BYTES = ctypes.sizeof(_hip.I8Args)
 _DTYPES = {torch.float32: _hip.RCV_F32, torch.bfloat16: _hip.RCV_BF16, torch.float16: _hip.RCV_F16}
 
 
@@ -69,7 +70,7 @@ def quantize_weight(w):
     return pack_codes(codes.clamp_(-127, 127).to(torch.int8).view(w.shape), scales)
 
 
-def _rows(t, what):
+def _rows(t):
     """A channels-last tensor as (tensor, number of rows, row pitch in elements); anything whose leading dimensions do not walk rows at
     one pitch is copied."""
     c = t.shape[-1]
@@ -92,18 +93,26 @@ def _rows(t, what):
     return t, t.numel() // c, c
 
 
-def _device(*tensors):
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError("rcvpose_amd runs on MI355X only: move the tensors to 'cuda' (no CPU fallback)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
+def _check_device(dev, *others):
+    """Every tensor of a call lives on `dev`."""
+    for t in others:
+        if t is not None and t.device != dev:
+            if not t.is_cuda:
+                _no_cpu()
             raise ValueError("all tensors of a call must be on one device")
-    return dev
+
+
+def _no_cpu():
+    _hip.lib()  # (raises first where no GPU is visible)
+    raise RuntimeError("rcvpose_amd runs on MI355X only: move the tensors to 'cuda' (no CPU fallback)")
+
+
+def _on_device(dev, call):
+    """call() with `dev` as the current device (the launch goes to dev's current stream)."""
+    if torch.cuda.current_device() == dev.index:
+        return call()
+    with torch.cuda.device(dev):
+        return call()
 
 
 def quantize_tokens(x, x1=None):
@@ -113,69 +122,82 @@ def quantize_tokens(x, x1=None):
     scale = float32(max |x| / 127) of the token, code = x / scale rounded half to even.  A token of zeros gets scale 0; a token with a
     NaN or an infinity gets scale NaN and codes 0, so products with it are NaN.  The rows of `codes` start 16 bytes aligned, as
     matmul and conv3x3 need them: for C not a multiple of 16 `codes` is a view of a wider buffer."""
-    L = _hip.lib()
-    if x.dtype not in _DTYPES or x.dim() < 1 or x.shape[-1] == 0:
+    L = _hip.load_library()
+    dtype, shape = _DTYPES.get(x.dtype), x.shape
+    if dtype is None or len(shape) < 1 or shape[-1] == 0:
         raise ValueError("tokens must be float32, bfloat16 or float16 [..., C] with at least one channel")
-    if x1 is not None and (x1.dtype != x.dtype or x1.shape[:-1] != x.shape[:-1] or x1.shape[-1] == 0):
+    if x1 is not None and (x1.dtype != x.dtype or x1.shape[:-1] != shape[:-1] or x1.shape[-1] == 0):
         raise ValueError("the second source must have the first one's type and leading dimensions")
-    c0, c1 = x.shape[-1], 0 if x1 is None else x1.shape[-1]
-    if c0 + c1 > MAX_CHANNELS:
+    c0, c1 = shape[-1], 0 if x1 is None else x1.shape[-1]
+    c = c0 + c1
+    if c > MAX_CHANNELS:
         raise ValueError("a token has at most %d channels" % MAX_CHANNELS)
-    dev = _device(x, x1)
-    with torch.cuda.device(dev):
-        x, rows, pitch0 = _rows(x, "tokens")
-        pitch1 = 0
-        if x1 is not None:
-            x1, _, pitch1 = _rows(x1, "tokens")
-        lead = x.shape[:-1]
-        pitch = (c0 + c1 + 15) // 16 * 16
-        codes = torch.empty(lead + (pitch,), dtype=torch.int8, device=dev)
-        scales = torch.empty(lead, dtype=torch.float32, device=dev)
-        if rows:
-            _hip.check(L.rcv_i8_quantize_tokens(x.data_ptr(), pitch0, c0, _hip.ptr(x1), pitch1, c1, _DTYPES[x.dtype], rows,
-                                                codes.data_ptr(), pitch, scales.data_ptr(), _hip.current_stream()),
-                       "rcv_i8_quantize_tokens")
-    return codes if pitch == c0 + c1 else codes[..., :c0 + c1], scales
+    if not x.is_cuda:
+        _no_cpu()
+    dev = x.device
+    _check_device(dev, x1)
+    x, rows, pitch0 = _rows(x)
+    pitch1, x1_ptr = 0, None
+    if x1 is not None:
+        x1, _, pitch1 = _rows(x1)
+        x1_ptr = x1.data_ptr()
+    pitch = (c + 15) // 16 * 16
+    codes = torch.empty(shape[:-1] + (pitch,), dtype=torch.int8, device=dev)
+    scales = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+    if rows:
+        rc = _on_device(dev, lambda: L.rcv_i8_quantize_tokens(x.data_ptr(), pitch0, c0, x1_ptr, pitch1, c1, dtype, rows, codes.data_ptr(), pitch,
+                                                              scales.data_ptr(), _hip.raw_stream(dev.index)))
+        if rc:
+            _hip.check(rc, "rcv_i8_quantize_tokens")
+    return codes if pitch == c else codes[..., :c], scales
 
 
-def _product(name, codes, scales, weight, bias, residual, relu, dtype, image):
-    L = _hip.lib()
-    k, n, lead = weight.channels, weight.out_channels, tuple(codes.shape[:-1])
-    if codes.dtype != torch.int8 or codes.dim() < 1 or codes.shape[-1] != k:
+def _product(name, codes, scales, weight, bias, residual, relu, dtype, height, width):
+    L = _hip.load_library()
+    k, n, shape = weight.channels, weight.out_channels, codes.shape
+    lead = shape[:-1]
+    if codes.dtype != torch.int8 or len(shape) < 1 or shape[-1] != k:
         raise ValueError("codes must be int8 [..., %d] for this weight" % k)
-    if scales.dtype != torch.float32 or tuple(scales.shape) != lead:
+    if scales.dtype != torch.float32 or scales.shape != lead:
         raise ValueError("scales must be float32 with one value per token")
-    if dtype not in _DTYPES:
+    out_type = _DTYPES.get(dtype)
+    if out_type is None:
         raise ValueError("output type must be torch.float32, torch.bfloat16 or torch.float16")
-    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (n,)):
-        raise ValueError("bias must be float32 [%d]" % n)
-    if residual is not None and (residual.dtype != dtype or tuple(residual.shape) != lead + (n,)):
-        raise ValueError("residual must have the output's type and shape")
-    dev = _device(codes, scales, weight.codes, bias, residual)
-    with torch.cuda.device(dev):
-        codes, rows, pitch = _rows(codes, "codes")
-        if rows == 1:  # (one row has no pitch of its own)
-            pitch = (k + 15) // 16 * 16
-        need = (rows - 1) * pitch + (k + 15) // 16 * 16
-        if rows and (pitch % 16 or codes.data_ptr() % 16 or codes.untyped_storage().nbytes() - codes.storage_offset() < need):
-            raise ValueError("token rows must start 16 bytes aligned and be readable up to a multiple of 16 channels: "
-                             "take the codes as quantize_tokens lays them out")
-        out = torch.empty(lead + (n,), dtype=dtype, device=dev)
-        if rows == 0:
-            return out
-        scales = scales.contiguous()
-        res_pitch = 0
-        if residual is not None:
-            residual, _, res_pitch = _rows(residual, "residual")
-        if bias is not None:
-            bias = bias.contiguous()
-        a = _hip.I8Args(ctypes.sizeof(_hip.I8Args), _DTYPES[dtype], codes.data_ptr(), scales.data_ptr(), weight.codes.data_ptr(),
-                        weight.scales.data_ptr(), None if bias is None else bias.data_ptr(),
-                        None if residual is None else residual.data_ptr(), out.data_ptr(), rows, pitch, res_pitch, n, k, n,
-                        image[0], image[1], int(bool(relu)), 0)
-        nbytes = getattr(L, name + "_workspace_bytes")(rows, k, n)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        _hip.check(getattr(L, name)(ctypes.byref(a), _hip.ptr(ws), nbytes, _hip.current_stream()), name)
+    if not codes.is_cuda:
+        _no_cpu()
+    dev = codes.device
+    _check_device(dev, scales, weight.codes, weight.scales, bias, residual)
+    out = torch.empty(lead + (n,), dtype=dtype, device=dev)
+    bias_ptr, res_ptr, res_pitch = None, None, 0
+    if bias is not None:
+        if bias.dtype != torch.float32 or bias.shape != (n,):
+            raise ValueError("bias must be float32 [%d]" % n)
+        bias = bias.contiguous()
+        bias_ptr = bias.data_ptr()
+    if residual is not None:
+        if residual.dtype != dtype or residual.shape != out.shape:
+            raise ValueError("residual must have the output's type and shape")
+        residual, _, res_pitch = _rows(residual)
+        res_ptr = residual.data_ptr()
+    codes, rows, pitch = _rows(codes)
+    if rows == 0:
+        return out
+    need = (k + 15) // 16 * 16
+    if rows == 1:  # (one row has no pitch of its own)
+        pitch = need
+    codes_ptr = codes.data_ptr()
+    if pitch % 16 or codes_ptr % 16 or codes.untyped_storage().nbytes() - codes.storage_offset() < (rows - 1) * pitch + need:
+        raise ValueError("token rows must start 16 bytes aligned and be readable up to a multiple of 16 channels: "
+                         "take the codes as quantize_tokens lays them out")
+    scales = scales.contiguous()
+    args = _hip.I8Args(_ARGS_BYTES, out_type, codes_ptr, scales.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(), bias_ptr, res_ptr,
+                       out.data_ptr(), rows, pitch, res_pitch, n, k, n, height, width, 1 if relu else 0, 0)
+    call, workspace_bytes = getattr(L, name), getattr(L, name + "_workspace_bytes")
+    nbytes = workspace_bytes(rows, k, n)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    rc = _on_device(dev, lambda: call(ctypes.byref(args), None if ws is None else ws.data_ptr(), nbytes, _hip.raw_stream(dev.index)))
+    if rc:
+        _hip.check(rc, name)
     return out
 
 
@@ -186,7 +208,7 @@ def matmul(codes, scales, weight, bias=None, residual=None, relu=False, dtype=to
     residual [..., N] of `dtype`.  The integer sums are exact; the result is rounded once, to `dtype`.  relu keeps a NaN."""
     if weight.taps != 1:
         raise ValueError("matmul takes a weight packed from [N, K]; a 3x3 weight belongs to conv3x3")
-    return _product("rcv_i8_matmul", codes, scales, weight, bias, residual, relu, dtype, (0, 0))
+    return _product("rcv_i8_matmul", codes, scales, weight, bias, residual, relu, dtype, 0, 0)
 
 
 def conv3x3(codes, scales, weight, bias=None, residual=None, relu=False, dtype=torch.bfloat16):
@@ -197,4 +219,4 @@ def conv3x3(codes, scales, weight, bias=None, residual=None, relu=False, dtype=t
         raise ValueError("conv3x3 takes a weight packed from [N, 3, 3, C]")
     if codes.dim() != 4:
         raise ValueError("codes must be int8 [B, H, W, C]")
-    return _product("rcv_i8_conv3x3", codes, scales, weight, bias, residual, relu, dtype, (int(codes.shape[1]), int(codes.shape[2])))
+    return _product("rcv_i8_conv3x3", codes, scales, weight, bias, residual, relu, dtype, codes.shape[1], codes.shape[2])
