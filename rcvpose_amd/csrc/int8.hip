@@ -23,6 +23,10 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 template <typename T> __device__ __forceinline__ float as_f32(T v) { return (float)v; }
 template <typename T> __device__ __forceinline__ T as_out(float v) { return (T)v; }
 
+// ---------------------------------------------------------------------------------------------
+// quantiser
+// ---------------------------------------------------------------------------------------------
+
 // round-half-even(x / s) of the exact quotient, s a normal number, |x| <= 127 s (1 + 2^-24): the product with 1/s is off by less
 // than one step, and the remainder x - q s is exact in one fma (it has no more significant bits than x and s share), so comparing
 // it with s / 2 settles the neighbours of a half.
@@ -34,33 +38,122 @@ __device__ __forceinline__ int quantize_exact(float x, float s, float inv)
     return (int)q;
 }
 
+// The bits of |x| as a 32-bit number that orders like |x|, NaNs above the infinity.
+template <typename T> __device__ __forceinline__ unsigned magnitude_bits(T v) { return __float_as_uint((float)v) & 0x7fffffffu; }
+
+// Sixteen channels c .. c + 15 of a token, zeros behind the last.  Rows may start anywhere: the vector loads of gfx950 need no alignment.
 template <typename T>
-__global__ __launch_bounds__(256) void k_i8_quantize(const T *x0, long long pitch0, int c0, const T *x1, long long pitch1, int c1,
-                                                     long long rows, int8_t *codes, long long codes_pitch, float *scales)
+__device__ __forceinline__ void load_chunk(T *v, const T *x0, int c0, const T *x1, int C, int c)
 {
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
+    struct __attribute__((packed)) Raw { T v[16]; };
+    if (c + 16 <= c0 || (c >= c0 && c + 16 <= C)) {
+        const Raw r = *(const Raw *)(c < c0 ? x0 + c : x1 + (c - c0));
+#pragma unroll
+        for (int e = 0; e < 16; e++) v[e] = r.v[e];
+    } else {
+        for (int e = 0; e < 16; e++) v[e] = c + e < c0 ? x0[c + e] : c + e < C ? x1[c + e - c0] : (T)0.f;
+    }
+}
+
+// The scale of a token from the largest magnitude's bits.
+__device__ __forceinline__ float token_scale(unsigned bits)
+{
+    if (bits >= 0x7f800000u) return __builtin_nanf("");
+    const float s = __fdiv_rn(__uint_as_float(bits), 127.f);
+    return s < 0x1p-126f ? 0.f : s;
+}
+
+// Codes of sixteen channels.  x / s + 1.5 * 2^23 in one fma leaves the code, rounded half to even, in the low byte; with 1/s rounded
+// the quotient is off by at most 127 * 2^-23 < 2^-15, so only a remainder within 2^-15 of a half can be wrong, and those (few)
+// chunks are done again exactly.
+template <typename T> __device__ __forceinline__ uint4 quantize_chunk(const T *v, float s, float inv)
+{
+    constexpr float MAGIC = 12582912.f;
+    unsigned w[4];
+    float d = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        const float x = as_f32(v[e]), m = fmaf(x, inv, MAGIC);
+        d = fmaxf(d, fabsf(fmaf(x, inv, MAGIC - m)));
+        const unsigned b = __float_as_uint(m) & 255u;
+        w[e >> 2] = e & 3 ? w[e >> 2] | b << (8 * (e & 3)) : b;
+    }
+    if (d > 0.5f - 0x1p-15f) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const unsigned b = (unsigned)quantize_exact(as_f32(v[e]), s, inv) & 255u;
+            w[e >> 2] = e & 3 ? w[e >> 2] | b << (8 * (e & 3)) : b;
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ void store_chunk(int8_t *codes, uint4 w, int C, int c, bool aligned)
+{
+    if (aligned && c + 16 <= C) *(uint4 *)(codes + c) = w;
+    else {
+        const unsigned *u = (const unsigned *)&w;
+        for (int e = 0; e < 16 && c + e < C; e++) codes[c + e] = (int8_t)(u[e >> 2] >> (8 * (e & 3)));
+    }
+}
+
+// L lanes per token, NV chunks of sixteen channels a lane: one pass, the token stays in registers.
+template <typename T, int L, int NV>
+__global__ __launch_bounds__(256) void k_i8_quantize(const T *x0, long long pitch0, int c0, const T *x1, long long pitch1, int c1,
+                                                     long long rows, int8_t *codes, long long codes_pitch, float *scales, bool aligned)
+{
+    const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / L;
+    const int lane = threadIdx.x % L, C = c0 + c1;
     if (row >= rows) return;
-    const int C = c0 + c1;
-    float amax = 0.f, poison = 0.f;
-    for (int c = lane; c < C; c += 64) {
-        const float v = as_f32(c < c0 ? x0[row * pitch0 + c] : x1[row * pitch1 + c - c0]);
-        amax = fmaxf(amax, fabsf(v));
-        poison += v * 0.f;  // NaN once v is a NaN or an infinity
+    T v[NV][16];
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int c = (i * L + lane) * 16;
+        if (c < C) load_chunk(v[i], x0 + row * pitch0, c0, x1 + row * pitch1, C, c);
+        else
+            for (int e = 0; e < 16; e++) v[i][e] = (T)0.f;
     }
-    for (int o = 32; o; o >>= 1) {
-        amax = fmaxf(amax, __shfl_xor(amax, o));
-        poison += __shfl_xor(poison, o);
-    }
-    float s = __fdiv_rn(amax, 127.f);
-    if (s < 0x1p-126f) s = 0.f;
-    if (poison != 0.f) s = __builtin_nanf("");  // (true for a NaN only: the sum of zeros is zero)
-    const float inv = s > 0.f ? 1.f / s : 0.f;
-    for (int c = lane; c < C; c += 64) {
-        const float v = as_f32(c < c0 ? x0[row * pitch0 + c] : x1[row * pitch1 + c - c0]);
-        codes[row * codes_pitch + c] = (int8_t)(s > 0.f ? quantize_exact(v, s, inv) : 0);
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) top = max(top, magnitude_bits(v[i][e]));
+#pragma unroll
+    for (int o = L / 2; o; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
+    const float s = token_scale(top), inv = s > 0.f ? 1.f / s : 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int c = (i * L + lane) * 16;
+        if (c < C) store_chunk(codes + row * codes_pitch, s > 0.f ? quantize_chunk(v[i], s, inv) : make_uint4(0u, 0u, 0u, 0u), C, c, aligned);
     }
     if (lane == 0) scales[row] = s;
+}
+
+// A workgroup per token of any length: the token is read twice, the second time from the caches.
+template <typename T>
+__global__ __launch_bounds__(1024) void k_i8_quantize_long(const T *x0, long long pitch0, int c0, const T *x1, long long pitch1, int c1,
+                                                           int8_t *codes, long long codes_pitch, float *scales, bool aligned)
+{
+    __shared__ unsigned tops[16];
+    const long long row = blockIdx.x;
+    const int C = c0 + c1;
+    T v[16];
+    unsigned top = 0;
+    for (int c = threadIdx.x * 16; c < C; c += 1024 * 16) {
+        load_chunk(v, x0 + row * pitch0, c0, x1 + row * pitch1, C, c);
+#pragma unroll
+        for (int e = 0; e < 16; e++) top = max(top, magnitude_bits(v[e]));
+    }
+    for (int o = 32; o; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
+    if (threadIdx.x % 64 == 0) tops[threadIdx.x / 64] = top;
+    __syncthreads();
+    for (int w = 0; w < 16; w++) top = max(top, tops[w]);
+    const float s = token_scale(top), inv = s > 0.f ? 1.f / s : 0.f;
+    for (int c = threadIdx.x * 16; c < C; c += 1024 * 16) {
+        load_chunk(v, x0 + row * pitch0, c0, x1 + row * pitch1, C, c);
+        store_chunk(codes + row * codes_pitch, s > 0.f ? quantize_chunk(v, s, inv) : make_uint4(0u, 0u, 0u, 0u), C, c, aligned);
+    }
+    if (threadIdx.x == 0) scales[row] = s;
 }
 
 // A view of memory for buffer loads: what lies beyond `bytes` reads as zeros.
@@ -587,11 +680,28 @@ __global__ __launch_bounds__(64 * S::NW, S::NW == 8 ? 2 : 1) void k_i8_tile(cons
     report_range<T>(p, vmax);
 }
 
-template <typename T> int launch_quantize(const void *x0, long long pitch0, int c0, const void *x1, long long pitch1, int c1, long long rows,
-                                          int8_t *codes, long long codes_pitch, float *scales, hipStream_t st)
+template <typename T>
+int launch_quantize(const void *x0_, long long pitch0, int c0, const void *x1_, long long pitch1, int c1, long long rows, int8_t *codes,
+                    long long codes_pitch, float *scales, hipStream_t st)
 {
-    hipLaunchKernelGGL((k_i8_quantize<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, (const T *)x0, pitch0, c0, (const T *)x1,
-                       pitch1, c1, rows, codes, codes_pitch, scales);
+    const T *x0 = (const T *)x0_, *x1 = (const T *)x1_;
+    const int C = c0 + c1;
+    const bool aligned = (uintptr_t)codes % 16 == 0 && codes_pitch % 16 == 0;
+#define RCV_I8_Q(L, NV)                                                                                                           \
+    if (C <= L * NV * 16) {                                                                                                       \
+        hipLaunchKernelGGL((k_i8_quantize<T, L, NV>), dim3((unsigned)((rows + 256 / L - 1) / (256 / L))), dim3(256), 0, st, x0, pitch0, c0, \
+                           x1, pitch1, c1, rows, codes, codes_pitch, scales, aligned);                                            \
+        RCV_LAUNCH_CHECK();                                                                                                       \
+        return RCV_OK;                                                                                                            \
+    }
+    RCV_I8_Q(4, 1)
+    RCV_I8_Q(16, 1)
+    RCV_I8_Q(64, 1)
+    RCV_I8_Q(64, 2)
+    RCV_I8_Q(64, 4)
+#undef RCV_I8_Q
+    hipLaunchKernelGGL((k_i8_quantize_long<T>), dim3((unsigned)rows), dim3(1024), 0, st, x0, pitch0, c0, x1, pitch1, c1, codes, codes_pitch,
+                       scales, aligned);
     RCV_LAUNCH_CHECK();
     return RCV_OK;
 }
@@ -753,7 +863,7 @@ int rcv_i8_quantize_tokens(const void *x0_dev, long long pitch0, int c0, const v
     if (c0 > I8_MAX_K || c1 > I8_MAX_K - c0 || rows > I8_MAX_ROWS) return RCV_E_TOO_LARGE;
     const int size = dtype == RCV_F32 ? 4 : 2;
     if ((uintptr_t)x0_dev % size || (uintptr_t)x1_dev % size || pitch0 < c0 || (c1 && pitch1 < c1) || codes_pitch < c0 + c1) return RCV_E_INVALID;
-    if (pitch0 > (1 << 24) || (c1 && pitch1 > (1 << 24)) || codes_pitch > (1 << 24) || rows > 4LL * 0x7fffffff) return RCV_E_TOO_LARGE;
+    if (pitch0 > (1 << 24) || (c1 && pitch1 > (1 << 24)) || codes_pitch > (1 << 24) || rows > 0x7fffffff) return RCV_E_TOO_LARGE;
     return i8_quantize(x0_dev, pitch0, c0, x1_dev, pitch1, c1, dtype, rows, codes_dev, codes_pitch, scales_dev, (hipStream_t)stream);
 }
 
