@@ -172,35 +172,54 @@ __device__ __forceinline__ i32x4 load16(__amdgpu_buffer_rsrc_t rsrc, int voff, i
     return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, voff, soff, 0));
 }
 
-// Four channels n .. n + 3 of token m: v = sum * sw + bias + residual, ReLU that keeps a NaN, rounded once to the output's type.
-// `v` holds the sums with the token scales applied.  Returns the largest magnitude stored.
-template <typename T> __device__ __forceinline__ float finish_quad(const I8Product &p, int g, long long m, int n, const float *v)
+// N consecutive channels of a row that may start anywhere (gfx950's vector accesses need no alignment)
+template <typename T, int N> struct Row {
+    typedef T Vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+template <typename T, int N> __device__ __forceinline__ typename Row<T, N>::Vec load_row(const T *x, int n, int Cout)
 {
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    const float *ws = p.weight_scales + (long long)g * p.weight_scale_gs + n, *bias = p.bias ? p.bias + (long long)g * p.bias_gs + n : nullptr;
-    const T *res = p.residual ? (const T *)p.residual + (long long)g * p.residual_gs + m * p.residual_pitch + n : nullptr;
+    typename Row<T, N>::Vec r = {};
+    if (n + N <= Cout) r = *(const typename Row<T, N>::Vec *)x;
+    else
+        for (int e = 0; e < N; e++) if (n + e < Cout) r[e] = x[e];
+    return r;
+}
+template <typename T> __device__ __forceinline__ const T *residual_row(const I8Product &p, int g, long long m)
+{
+    return p.residual ? (const T *)p.residual + (long long)g * p.residual_gs + m * p.residual_pitch : nullptr;
+}
+// Channels n .. n + N - 1 of token m, scaled and with the bias: residual, ReLU that keeps a NaN, rounded once to the output's type.  Returns
+// the largest magnitude stored.
+template <typename T, int N>
+__device__ __forceinline__ float finish_row(const I8Product &p, int g, long long m, int n, float *v, typename Row<T, N>::Vec res)
+{
     T *out = (T *)p.out + (long long)g * p.out_gs + m * p.out_pitch + n;
-    const bool whole = p.vec && n + 3 < p.Cout;
-    T4 r = T4{}, o;
-    if (res) {
-        if (whole) r = *(const T4 *)res;
-        else
-            for (int e = 0; e < 4; e++) if (n + e < p.Cout) r[e] = res[e];
-    }
     float vmax = 0.f;
+    typename Row<T, N>::Vec o;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+        if (p.residual) v[e] += as_f32(res[e]);
+        if (p.relu) v[e] = v[e] < 0.f ? 0.f : v[e];
+        if (n + e < p.Cout) vmax = fmaxf(vmax, fabsf(v[e]));
+        o[e] = as_out<T>(v[e]);
+    }
+    if (n + N <= p.Cout) *(typename Row<T, N>::Vec *)out = o;
+    else
+        for (int e = 0; e < N; e++) if (n + e < p.Cout) out[e] = o[e];
+    return vmax;
+}
+// Four channels whose sums still lack the weight scales and the bias.
+template <typename T> __device__ __forceinline__ float finish_quad(const I8Product &p, int g, long long m, int n, const float *sum)
+{
+    const float *ws = p.weight_scales + (long long)g * p.weight_scale_gs + n, *bias = p.bias ? p.bias + (long long)g * p.bias_gs + n : nullptr;
+    float v[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         const bool live = n + e < p.Cout;
-        float y = fmaf(v[e], live ? ws[e] : 0.f, live && bias ? bias[e] : 0.f);
-        if (res) y += as_f32(r[e]);
-        if (p.relu) y = y < 0.f ? 0.f : y;
-        if (live) vmax = fmaxf(vmax, fabsf(y));
-        o[e] = as_out<T>(y);
+        v[e] = fmaf(sum[e], live ? ws[e] : 0.f, live && bias ? bias[e] : 0.f);
     }
-    if (whole) *(T4 *)out = o;
-    else
-        for (int e = 0; e < 4; e++) if (n + e < p.Cout) out[e] = o[e];
-    return vmax;
+    const T *res = residual_row<T>(p, g, m);
+    return finish_row<T, 4>(p, g, m, n, v, res ? load_row<T, 4>(res + n, n, p.Cout) : typename Row<T, 4>::Vec{});
 }
 template <typename T> __device__ __forceinline__ void report_range(const I8Product &p, float vmax)
 {
@@ -404,25 +423,33 @@ template <int I, int N, typename F> __device__ __forceinline__ void for_each(F &
     }
 }
 
-template <int TAPS_, int WT_, int WC_, int TT_, int CT_, int KB_, int NST_> struct TileShape {
-    static constexpr int TAPS = TAPS_, WT = WT_, WC = WC_, TT = TT_, CT = CT_, KB = KB_, NST = NST_;
+template <int TAPS_, int WT_, int WC_, int TT_, int CT_, int NA_, int NB_, bool SPLIT_ = false> struct TileShape {
+    static constexpr bool SPLIT = SPLIT_;  // the sum may be divided over workgroups
+    static constexpr int TAPS = TAPS_, WT = WT_, WC = WC_, TT = TT_, CT = CT_, NA = NA_, NB = NB_;
+    static constexpr int KB = 128;                                // codes of a row per step: one cache line
     static constexpr int NW = WT * WC, BM = WT * TT * 16, BN = WC * CT * 16;
-    static constexpr int RPP = 1024 / KB;                         // rows of one piece
-    static constexpr int PA = BM / RPP / NW, PB = BN / RPP / NW;  // pieces of a wave per step
-    static constexpr int P = PA + PB, STAGE = (BM + BN) * KB;
-    static constexpr int LDS = NST * STAGE + (TAPS == 9 ? 9 * BM * 4 : 0);
-    static_assert(BM % (RPP * NW) == 0 && BN % (RPP * NW) == 0 && LDS <= 160 * 1024 && (KB == 64 || KB == 128), "tile plan");
-    static_assert(TAPS == 1 || KB == 128, "a tap is a whole number of fragment pairs");
+    static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;      // pieces (8 rows) of a wave per step
+    static constexpr int A_BYTES = BM * KB, B_BYTES = BN * KB, B_RING = NA * A_BYTES, TABLE = B_RING + NB * B_BYTES;
+    static constexpr int LDS = TABLE + (TAPS == 9 ? 9 * BM * 4 : 0);
+    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && LDS <= 160 * 1024 && NA >= 3 && NB >= 2 && NB <= NA, "tile plan");
+    // Pieces in order of issue, per step kt: the tokens of step kt + NA - 1 in its first half, the weights of step kt + NB in its second.
+    // Half-way through step kt everything of step kt + 1 has to be there: what may still be on its way was issued later.
+    static constexpr int LATE = NB == NA ? (NA - 2) * (PA + PB) : (NB - 2) * (PA + PB) + PA;
 };
 
 // BM tokens x BN channels per workgroup, WT x WC waves of TT x CT 16 x 16 tiles.  The weights are the matrix instruction's first operand, so a
-// lane ends up with four consecutive channels of one token.  A ring of NST stages of KB codes per row, filled NST - 1 steps ahead; rows are
-// KB bytes and the 16-byte chunks of a row are permuted (chunk ^= row bits) on the way in, so that the sixteen rows of a fragment
-// read fall on all banks.  One barrier per step.
+// lane ends up with four consecutive channels of one token.  Rings of NA token and NB weight stages of 128 codes a row; the eight 16-byte
+// chunks of a row are permuted (chunk ^= row bits) on the way in, so that the sixteen rows of a fragment read fall on all banks.
+// One barrier per step, half-way: before it a wave has read the step's last fragments, behind it the next step's first are there.
+//
+// TAPS = 9 walks tap by tap; after every tap the integer sums are scaled into `sum`.
+//
+// gridDim.y > 1 divides the sum: a workgroup takes its share of the channels (TAPS = 1) or of the taps and leaves raw sums in `partial`
+// [split][group][rows][quads of channels] for k_i8_finish.
 template <typename T, typename S>
-__global__ __launch_bounds__(64 * S::NW, S::NW == 8 ? 2 : 1) void k_i8_tile(const I8Product p, int tiles_m, int tiles_n)
+__global__ __launch_bounds__(64 * S::NW, 2) void k_i8_tile(const I8Product p, int tiles_m, int tiles_n, f32x4 *partial)
 {
-    constexpr int TAPS = S::TAPS, TT = S::TT, CT = S::CT, KB = S::KB, NST = S::NST, PA = S::PA, P = S::P, BM = S::BM, BN = S::BN;
+    constexpr int TAPS = S::TAPS, TT = S::TT, CT = S::CT, KB = S::KB, PA = S::PA, PB = S::PB, BM = S::BM, BN = S::BN;
     constexpr int OOB = (int)0x80000000;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)smem;
@@ -453,6 +480,7 @@ __global__ __launch_bounds__(64 * S::NW, S::NW == 8 ? 2 : 1) void k_i8_tile(cons
     // which of the nine taps of a token lie inside its image
     const int W = p.W, H = p.H;
     int x0 = 0, y0 = 0;
+    const float rw = 1.f / (float)max(W, 1), rh = 1.f / (float)max(H, 1);
     if constexpr (TAPS == 9) {
         const long long l = m0 / W;
         x0 = __builtin_amdgcn_readfirstlane((int)(m0 - l * W));
@@ -460,11 +488,112 @@ __global__ __launch_bounds__(64 * S::NW, S::NW == 8 ? 2 : 1) void k_i8_tile(cons
     }
     auto taps_inside = [&](int row) -> unsigned {
         if (row >= left) return 0u;
-        const int t = x0 + row, l = t / W, x = t - l * W, y = (y0 + l) % H;
+        // (a product with the reciprocal, half a step up: the quotient is at most BM for W = 1 and 1 for the widest image, its error far
+        // below the half step's distance 1 / (2 W) to a whole number)
+        const int t = x0 + row, l = (int)(((float)t + 0.5f) * rw), x = t - l * W, yl = y0 + l, y = yl - (int)(((float)yl + 0.5f) * rh) * H;
         const unsigned cols = (x > 0 ? 1u : 0u) | 2u | (x + 1 < W ? 4u : 0u);
         return (y > 0 ? cols : 0u) | cols << 3 | (y + 1 < H ? cols << 6 : 0u);
     };
-    float *sa_tab = (float *)(smem + NST * S::STAGE);  // [9][BM]: the scale under which a token's tap enters, 0 outside the image
+    // What the epilogue needs, requested first: the scales of this lane's tokens, the scales and biases of the V channels it will finish.
+    constexpr int V = 16 / sizeof(T), CPR = BN / V;
+    constexpr bool LATE_SCALES = TT * CT > 16 && TAPS == 1;  // (no registers to keep them over the loop)
+    const int c = tid % CPR, n = n0 + c * V;
+    float sa[TT] = {};
+    typename Row<float, V>::Vec sw = {}, bias = {};
+    auto load_scales = [&]() {
+        if constexpr (!S::SPLIT) {
+#pragma unroll
+            for (int j = 0; j < TT; j++) {
+                const int row = wt * TT * 16 + j * 16 + r16;
+                sa[j] = TAPS == 1 && row < left ? cs[m0 + row] : 0.f;
+            }
+            sw = load_row<float, V>(p.weight_scales + (long long)g * p.weight_scale_gs + n, n, p.Cout);
+            if (p.bias) bias = load_row<float, V>(p.bias + (long long)g * p.bias_gs + n, n, p.Cout);
+        }
+    };
+    if constexpr (!LATE_SCALES) load_scales();
+
+    // this lane's part of the pieces: row lane / 8 of the piece, 16-byte slot lane % 8
+    auto chunk_of = [&](int row, int slot) { return slot ^ ((row >> 1) & 7); };
+    int aoff[PA], boff[PB];
+    unsigned inside[TAPS == 9 ? PA : 1];
+#pragma unroll
+    for (int c = 0; c < PA; c++) {
+        const int row = (wave * PA + c) * 8 + lane / 8;
+        aoff[c] = row < left ? (int)(row * p.code_pitch) + chunk_of(row, lane % 8) * 16 : OOB;
+        if constexpr (TAPS == 9) inside[c] = taps_inside(row);
+    }
+#pragma unroll
+    for (int c = 0; c < PB; c++) {
+        const int row = (wave * PB + c) * 8 + lane / 8;
+        boff[c] = row * wrow + chunk_of(row, lane % 8) * 16;
+    }
+
+    // Where the next token and the next weight pieces come from.  Behind the last step the pieces go on with every lane out of range, which
+    // keeps the counts the same.
+    const long long pitch = p.code_pitch;
+    const int units = TAPS == 9 ? 9 : (p.K + KB - 1) / KB;  // what a split takes a run of
+    const int u0 = S::SPLIT ? (int)(units * blockIdx.y / gridDim.y) : 0, u1 = S::SPLIT ? (int)(units * (blockIdx.y + 1) / gridDim.y) : units;
+    const int tap0 = TAPS == 9 ? u0 : 0, tap1 = TAPS == 9 ? u1 : 1;
+    const int klo = TAPS == 9 ? 0 : u0 * KB, khi = TAPS == 9 ? (p.K + KB - 1) / KB * KB : u1 * KB;
+    struct Walk { int tap, k, done; };
+    auto step = [&](Walk &w) -> bool {  // true where another tap begins
+        w.k += KB;
+        if (w.k < khi) return false;
+        w.k = klo;
+        if constexpr (TAPS == 9) {
+            w.tap++;
+            if (w.tap < tap1) return true;
+            w.tap = tap0;
+        }
+        w.done = OOB;
+        return false;
+    };
+    Walk ia{tap0, klo, 0}, ib{tap0, klo, 0};
+    i32x4 ra, rb;
+    unsigned a_lds = lds0 + wave * PA * 1024, b_lds = lds0 + S::B_RING + wave * PB * 1024;
+    const unsigned a_last = a_lds + (S::NA - 1) * S::A_BYTES, b_last = b_lds + (S::NB - 1) * S::B_BYTES;
+    auto a_tap = [&]() {
+        const int8_t *a = codes + (m0 + (TAPS == 9 ? (long long)(ia.tap / 3 - 1) * W + (ia.tap % 3 - 1) : 0)) * pitch;
+        ra = descriptor(a, codes_end - a);
+    };
+    auto b_tap = [&]() { rb = descriptor(wts + (long long)ib.tap * p.kp, wbytes - (long long)ib.tap * p.kp); };
+    auto a_piece = [&](auto cc) {
+        constexpr int c = decltype(cc)::value;
+        int v = aoff[c];
+        if constexpr (TAPS == 9) v = (inside[c] >> ia.tap) & 1u ? v : OOB;
+        dma16<c * 1024>(ra, ia.k, a_lds, v | ia.done);
+    };
+    auto b_piece = [&](auto cc) {
+        constexpr int c = decltype(cc)::value;
+        dma16<c * 1024>(rb, ib.k, b_lds, boff[c] | ib.done);
+    };
+    auto a_end = [&]() {
+        a_lds = a_lds == a_last ? a_last - (S::NA - 1) * S::A_BYTES : a_lds + S::A_BYTES;
+        if (step(ia)) a_tap();
+    };
+    auto b_end = [&]() {
+        b_lds = b_lds == b_last ? b_last - (S::NB - 1) * S::B_BYTES : b_lds + S::B_BYTES;
+        if (step(ib)) b_tap();
+    };
+
+    a_tap();
+    b_tap();
+    asm volatile("s_nop 4");  // (scalars that came through vector registers, before the first piece reads them)
+    for (int s = 0; s < S::NA - 1; s++) {  // tokens of steps 0 .. NA - 2 and weights of steps 0 .. NB - 1 in the order of the loop
+        for_each<0, PA>(a_piece);
+        a_end();
+        if (s >= S::NA - 1 - S::NB) {
+            for_each<0, PB>(b_piece);
+            b_end();
+        }
+    }
+    if constexpr (S::NB == S::NA) {
+        for_each<0, PB>(b_piece);
+        b_end();
+    }
+
+    float *sa_tab = (float *)(smem + S::TABLE);  // [9][BM]: the scale under which a token's tap enters, 0 outside the image
     if constexpr (TAPS == 9) {
         for (int row = tid; row < BM; row += 64 * S::NW) {
             const unsigned ok = taps_inside(row);
@@ -472,64 +601,6 @@ __global__ __launch_bounds__(64 * S::NW, S::NW == 8 ? 2 : 1) void k_i8_tile(cons
             for (int t = 0; t < 9; t++)
                 sa_tab[t * BM + row] = (ok >> t) & 1u ? cs[m0 + row + (long long)(t / 3 - 1) * W + (t % 3 - 1)] : 0.f;
         }
-    }
-
-    // this lane's part of the pieces: row lane / (KB / 16) of the piece, 16-byte slot lane % (KB / 16)
-    constexpr int LPR = KB / 16;
-    auto chunk_of = [&](int row, int slot) { return KB == 128 ? slot ^ ((row >> 1) & 7) : slot ^ (-(row >> 2) & 3); };
-    int voff[P];
-    unsigned inside[TAPS == 9 ? PA : 1];
-#pragma unroll
-    for (int c = 0; c < P; c++) {
-        const bool tok = c < PA;
-        const int row = (tok ? wave * PA + c : wave * S::PB + c - PA) * S::RPP + lane / LPR;
-        const int chunk = chunk_of(row, lane % LPR) * 16;
-        if (tok) {
-            voff[c] = row < left ? (int)(row * p.code_pitch) + chunk : OOB;
-            if constexpr (TAPS == 9) inside[c] = taps_inside(row);
-        } else
-            voff[c] = row * wrow + chunk;
-    }
-
-    // The step being issued.  Behind the last step the pieces go on with every lane out of range (`done`), which keeps the counts the same.
-    const int ksteps = KB == 64 ? p.kp / KB : (p.K + KB - 1) / KB, nk = TAPS * ksteps;  // (pairs of steps: the weights are zero up to kp)
-    const long long pitch = p.code_pitch;
-    int i_tap = 0, i_k = 0, i_left = nk, done = 0;
-    unsigned i_lds = lds0 + wave * PA * 1024;
-    const unsigned lds_w = BM * KB + (wave * S::PB - wave * PA) * 1024, lds_end = i_lds + NST * S::STAGE;
-    i32x4 ra, rw;
-    auto begin_tap = [&]() {
-        const int8_t *a = codes + (m0 + (TAPS == 9 ? (long long)(i_tap / 3 - 1) * W + (i_tap % 3 - 1) : 0)) * pitch;
-        ra = descriptor(a, codes_end - a);
-        rw = descriptor(wts + (long long)i_tap * p.kp, wbytes - (long long)i_tap * p.kp);
-    };
-    auto piece = [&](auto cc) {
-        constexpr int c = decltype(cc)::value;
-        if constexpr (c < PA) {
-            int v = voff[c];
-            if constexpr (TAPS == 9) v = (inside[c] >> i_tap) & 1u ? v : OOB;  // (no bit is set behind the ninth tap)
-            else v |= done;
-            dma16<c * 1024>(ra, i_k, i_lds, v);
-        } else
-            dma16<(c - PA) * 1024>(rw, i_k, i_lds + lds_w, voff[c] | done);
-    };
-    auto end_step = [&]() {
-        i_lds = i_lds + S::STAGE == lds_end ? lds_end - NST * S::STAGE : i_lds + S::STAGE;
-        i_left--;
-        done = i_left > 0 ? 0 : OOB;
-        i_k += KB;
-        if (TAPS == 9 && i_k == ksteps * KB) {
-            i_k = 0;
-            i_tap++;
-            if (i_tap < 9) begin_tap();
-        }
-    };
-
-    begin_tap();
-    asm volatile("s_nop 4");  // (scalars that came through vector registers, before the first piece reads them)
-    for (int s = 0; s < NST; s++) {
-        for_each<0, P>(piece);
-        end_step();
     }
 
     i32x4 acc[CT][TT];
@@ -542,23 +613,22 @@ __global__ __launch_bounds__(64 * S::NW, S::NW == 8 ? 2 : 1) void k_i8_tile(cons
             if constexpr (TAPS == 9) sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
     i32x4 tf[2][TT], wf[2][CT];
-    const int t_row = (wt * TT * 16 + r16) * KB, w_row = BM * KB + (wc * CT * 16 + r16) * KB;
-    int r_stage = 0;  // byte offset of the stage being read
+    const int t_row = (wt * TT * 16 + r16) * KB, w_row = S::B_RING + (wc * CT * 16 + r16) * KB;
+    int a_stage = 0, b_stage = 0;  // byte offsets of the stages being read
     auto read = [&](int f, int half, int q) {  // fragment q of set f
         const int slot = chunk_of(r16, half * 4 + kq) * 16;
-        if (q < TT) tf[f][q] = *(const i32x4 *)(smem + r_stage + t_row + slot + q * 16 * KB);
-        else wf[f][q - TT] = *(const i32x4 *)(smem + r_stage + w_row + slot + (q - TT) * 16 * KB);
+        if (q < TT) tf[f][q] = *(const i32x4 *)(smem + a_stage + t_row + slot + q * 16 * KB);
+        else wf[f][q - TT] = *(const i32x4 *)(smem + b_stage + w_row + slot + (q - TT) * 16 * KB);
     };
-    auto next_stage = [&]() { r_stage = r_stage + S::STAGE == NST * S::STAGE ? 0 : r_stage + S::STAGE; };
-    // all products of fragment set f; meanwhile the other set is read (from `half` of the current read stage) and pieces [lo, hi) are issued
-    constexpr int NM = TT * CT, NF = TT + CT, SEG = NM / 4;
-    auto multiply = [&](auto ff, int half, auto lo_, auto hi_) {
-        constexpr int f = decltype(ff)::value, lo = decltype(lo_)::value, hi = decltype(hi_)::value;
+    // all products of fragment set f; meanwhile the other set is read from `half` of the current stages and N pieces are issued
+    constexpr int NM = TT * CT, NF = TT + CT, SEG = NM / 4, RSEG = SEG / 2;  // (the reads go into the first half: they are back before the barrier)
+    auto multiply = [&](auto ff, int half, auto count, auto &&piece) {
+        constexpr int f = decltype(ff)::value, n = decltype(count)::value;
         for_each<0, SEG>([&](auto ss) {
             constexpr int s = decltype(ss)::value;
 #pragma unroll
-            for (int q = s * NF / SEG; q < (s + 1) * NF / SEG; q++) read(1 - f, half, q);
-            for_each<lo + s * (hi - lo) / SEG, lo + (s + 1) * (hi - lo) / SEG>(piece);
+            for (int q = 0; q < NF; q++) if (q * RSEG / NF == s) read(1 - f, half, q);
+            for_each<s * n / SEG, (s + 1) * n / SEG>(piece);
 #pragma unroll
             for (int e = s * 4; e < s * 4 + 4; e++) {
                 const int i = e / TT, j = e % TT;
@@ -569,113 +639,98 @@ __global__ __launch_bounds__(64 * S::NW, S::NW == 8 ? 2 : 1) void k_i8_tile(cons
     };
     constexpr std::integral_constant<int, 0> c0{};
     constexpr std::integral_constant<int, 1> c1{};
-    constexpr std::integral_constant<int, P / 2> ch{};
-    constexpr std::integral_constant<int, P> cp{};
+    constexpr std::integral_constant<int, PA> pa{};
+    constexpr std::integral_constant<int, PB> pb{};
 
-    wait_pieces<P *(NST - 1)>();
+    wait_pieces<S::LATE + PB>();
     __builtin_amdgcn_s_barrier();
 #pragma unroll
     for (int q = 0; q < NF; q++) read(0, 0, q);
-    if constexpr (KB == 128) {
-        // a step's pieces are spread over its second half and the next step's first
-        bool first = true;
-        for (int tap = 0; tap < TAPS; tap++) {
-            for (int ks = 0; ks < ksteps; ks++) {
-                if (first) multiply(c0, 1, cp, cp);
-                else {
-                    multiply(c0, 1, ch, cp);
-                    end_step();
-                }
-                first = false;
-                wait_pieces<P *(NST - 2)>();  // the next stage is here; nobody reads the current one any more
-                __builtin_amdgcn_s_barrier();
-                next_stage();
-                multiply(c1, 0, c0, ch);
-            }
-            if constexpr (TAPS == 9) {
-#pragma unroll
-                for (int j = 0; j < TT; j++) {
-                    const float sa = sa_tab[tap * BM + wt * TT * 16 + j * 16 + r16];
-#pragma unroll
-                    for (int i = 0; i < CT; i++) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) sum[i][j][e] = fmaf((float)acc[i][j][e], sa, sum[i][j][e]);
-                        acc[i][j] = i32x4{0, 0, 0, 0};
-                    }
-                }
-            }
+    for (int tap = tap0; tap < tap1; tap++) {
+        for (int k = klo; k < khi; k += KB) {
+            multiply(c0, 1, pa, a_piece);
+            a_end();
+            wait_pieces<S::LATE>();  // the next step is here; nobody reads the current one any more
+            __builtin_amdgcn_s_barrier();
+            a_stage = a_stage == (S::NA - 1) * S::A_BYTES ? 0 : a_stage + S::A_BYTES;
+            b_stage = b_stage == (S::NB - 1) * S::B_BYTES ? 0 : b_stage + S::B_BYTES;
+            multiply(c1, 0, pb, b_piece);
+            b_end();
         }
-    } else {
-        for (int ks = 0; ks < nk; ks += 2) {
-            for_each<0, 2>([&](auto f) {
-                wait_pieces<P *(NST - 2)>();
-                __builtin_amdgcn_s_barrier();
-                next_stage();
-                multiply(f, 0, c0, cp);
-                end_step();
-            });
+        if constexpr (TAPS == 9) {
+#pragma unroll
+            for (int j = 0; j < TT; j++) {
+                const float sa = sa_tab[tap * BM + wt * TT * 16 + j * 16 + r16];
+#pragma unroll
+                for (int i = 0; i < CT; i++) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sum[i][j][e] = fmaf((float)acc[i][j][e], sa, sum[i][j][e]);
+                    acc[i][j] = i32x4{0, 0, 0, 0};
+                }
+            }
         }
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // (the last pieces: zeros nobody reads)
 
-    // epilogue: four channels of a token at a time, straight from the registers
-    typedef T T4 __attribute__((ext_vector_type(4)));
+    if constexpr (LATE_SCALES) load_scales();
+    // Epilogue: the scaled sums go through LDS, so that rows leave (and the residual's rows come) in whole lines.
+    constexpr int SROW = BN + 4, ROUND = 64 * S::NW / CPR;
+    static_assert(BM * SROW * 4 <= S::LDS || S::TAPS == 1, "the tile fits");
+    constexpr int PARTS = BM * SROW * 4 <= S::LDS ? 1 : 2, PROWS = BM / PARTS;
+    float *stage = (float *)smem;
     float vmax = 0.f;
-    T *out = (T *)p.out + (long long)g * p.out_gs;
-    const T *res = p.residual ? (const T *)p.residual + (long long)g * p.residual_gs : nullptr;
-    const float *bias = p.bias ? p.bias + (long long)g * p.bias_gs : nullptr, *ws = p.weight_scales + (long long)g * p.weight_scale_gs;
-    float sa[TT];
 #pragma unroll
-    for (int j = 0; j < TT; j++) {
-        const int row = wt * TT * 16 + j * 16 + r16;
-        sa[j] = TAPS == 1 && row < left ? cs[m0 + row] : 0.f;
-    }
+    for (int part = 0; part < PARTS; part++) {
+        __syncthreads();  // the ring (the part before) has been read
+        if (PARTS == 1 || wt * TT * 16 / PROWS == part) {
 #pragma unroll
-    for (int i = 0; i < CT; i++) {
-        const int n = n0 + (wc * CT + i) * 16 + kq * 4;
-        float b4[4], s4[4];
+            for (int i = 0; i < CT; i++) {
+                const int col = (wc * CT + i) * 16 + kq * 4;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            b4[e] = bias && n + e < p.Cout ? bias[n + e] : 0.f;
-            s4[e] = n + e < p.Cout ? ws[n + e] : 0.f;
-        }
-        const bool whole = p.vec && n + 3 < p.Cout;
-        T4 r4[TT];
+                for (int j = 0; j < TT; j++) {
+                    const int row = wt * TT * 16 + j * 16 + r16;
+                    f32x4 v;
 #pragma unroll
-        for (int j = 0; j < TT; j++) {
-            const int row = wt * TT * 16 + j * 16 + r16;
-            const long long at = (m0 + row) * p.residual_pitch + n;
-            r4[j] = T4{};
-            if (!res || row >= left) continue;
-            if (whole) r4[j] = *(const T4 *)(res + at);
-            else {
-#pragma unroll
-                for (int e = 0; e < 4; e++) if (n + e < p.Cout) r4[j][e] = res[at + e];
+                    for (int e = 0; e < 4; e++) {
+                        if constexpr (TAPS == 9) v[e] = sum[i][j][e];
+                        else v[e] = S::SPLIT ? __int_as_float(acc[i][j][e]) : (float)acc[i][j][e] * sa[j];
+                    }
+                    *(f32x4 *)(stage + (row - part * PROWS) * SROW + col) = v;
+                }
             }
         }
-#pragma unroll
-        for (int j = 0; j < TT; j++) {
-            const int row = wt * TT * 16 + j * 16 + r16;
-            const long long at = (m0 + row) * p.out_pitch + n;
-            T4 o;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                float v;
-                if constexpr (TAPS == 9) v = sum[i][j][e];
-                else v = (float)acc[i][j][e] * sa[j];
-                v = fmaf(v, s4[e], b4[e]);
-                if (res) v += as_f32(r4[j][e]);
-                if (p.relu) v = v < 0.f ? 0.f : v;  // (a NaN stays)
-                if (row < left && n + e < p.Cout) vmax = fmaxf(vmax, fabsf(v));
-                o[e] = as_out<T>(v);
+        __syncthreads();
+        constexpr int AHEAD = 4;  // residual rows requested together
+        static_assert(PROWS % (ROUND * AHEAD) == 0, "whole rounds");
+        if constexpr (S::SPLIT) {  // raw sums: float32 (TAPS = 9) or integers
+            const long long quads = (p.Cout + 3) / 4;
+            for (int r = tid / (BN / 4); r < PROWS; r += 64 * S::NW / (BN / 4)) {
+                const int row = part * PROWS + r, col = tid % (BN / 4);
+                if (row < left && n0 + col * 4 < p.Cout)
+                    partial[(((long long)blockIdx.y * p.groups + g) * p.rows + m0 + row) * quads + n0 / 4 + col] = *(const f32x4 *)(stage + r * SROW + col * 4);
             }
-            if (row >= left) continue;
-            if (whole) *(T4 *)(out + at) = o;
-            else {
+        } else if (n < p.Cout)
+            for (int r0 = tid / CPR; r0 < PROWS; r0 += ROUND * AHEAD) {
+                typename Row<T, V>::Vec res[AHEAD] = {};
+                if (p.residual) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) if (n + e < p.Cout) out[at + e] = o[e];
+                    for (int a = 0; a < AHEAD; a++) {
+                        const int row = part * PROWS + r0 + a * ROUND;
+                        if (row < left) res[a] = load_row<T, V>(residual_row<T>(p, g, m0 + row) + n, n, p.Cout);
+                    }
+                }
+#pragma unroll
+                for (int a = 0; a < AHEAD; a++) {
+                    const int r = r0 + a * ROUND, row = part * PROWS + r;
+                    if (row >= left) continue;
+                    float v[V];
+#pragma unroll
+                    for (int q = 0; q < V / 4; q++) *(f32x4 *)(v + 4 * q) = *(const f32x4 *)(stage + r * SROW + c * V + 4 * q);
+#pragma unroll
+                    for (int e = 0; e < V; e++) v[e] = fmaf(v[e], sw[e], bias[e]);
+                    vmax = fmaxf(vmax, finish_row<T, V>(p, g, m0 + row, n, v, res[a]));
+                }
             }
-        }
     }
     report_range<T>(p, vmax);
 }
@@ -696,6 +751,7 @@ int launch_quantize(const void *x0_, long long pitch0, int c0, const void *x1_, 
     }
     RCV_I8_Q(4, 1)
     RCV_I8_Q(16, 1)
+    RCV_I8_Q(32, 1)
     RCV_I8_Q(64, 1)
     RCV_I8_Q(64, 2)
     RCV_I8_Q(64, 4)
@@ -717,42 +773,69 @@ int allow_lds(const void *kernel, int bytes, std::atomic<unsigned long long> &re
     return RCV_OK;
 }
 
-template <typename T, typename S> int launch_tile(const I8Product &p, hipStream_t st)
+// How a product runs.
+struct Plan {
+    enum Kind { WIDE, TALL, SQUARE, NARROW, DIRECT } kind;
+    int splits;
+    size_t bytes;  // of partial sums
+};
+
+long long tile_count(long long rows, int Cout, int groups, int bm, int bn) { return ((rows + bm - 1) / bm) * ((Cout + bn - 1) / bn) * groups; }
+
+Plan plan_product(long long rows, int K, int Cout, int taps, int groups)
+{
+    Plan pl{Plan::SQUARE, 1, 0};
+    const int steps = taps * ((K + 127) / 128);
+    if (rows <= 64) {
+        pl.kind = Plan::DIRECT;
+        const long long wgs = tile_count(rows, Cout, groups, 64, 16);
+        while (wgs * pl.splits * 2 <= 256 && steps >= pl.splits * 2 * 16) pl.splits *= 2;  // (at least four 64-channel steps a wave)
+    } else {
+        // rounds of the chip's 256 CUs times the relative time of a tile
+        auto cost = [&](int bm, int bn, double w) { return (double)((tile_count(rows, Cout, groups, bm, bn) + 255) / 256) * w; };
+        if (taps == 1) {
+            const long long wide = tile_count(rows, Cout, groups, 256, 256);
+            if (K >= 1024 && wide * 4 >= 3 * ((wide + 255) / 256 * 256)) pl.kind = Plan::WIDE;
+        } else if (Cout <= 64) {
+            if (cost(256, 64, 0.66) <= cost(128, 128, 0.62)) pl.kind = Plan::NARROW;
+        } else if (cost(256, 128, 1.0) <= cost(128, 128, 0.62))
+            pl.kind = Plan::TALL;
+        if (pl.kind == Plan::SQUARE && steps >= 48) {
+            const long long wgs = tile_count(rows, Cout, groups, 128, 128);
+            if (taps == 9) pl.splits = wgs * 9 <= 288 ? 9 : wgs * 3 <= 288 ? 3 : 1;
+            else
+                while (wgs * pl.splits * 2 <= 288 && steps >= pl.splits * 2 * 16) pl.splits *= 2;
+        }
+    }
+    if (pl.splits > 1) pl.bytes = (size_t)pl.splits * groups * rows * ((Cout + 3) / 4) * 16;
+    return pl;
+}
+
+template <typename T, int TAPS> int launch_finish(const I8Product &p, const Plan &pl, const void *partial, hipStream_t st)
+{
+    const long long quads = p.rows * ((p.Cout + 3) / 4);
+    hipLaunchKernelGGL((k_i8_finish<T, TAPS>), dim3((unsigned)((quads + 255) / 256), 1, p.groups), dim3(256), 0, st, p, (const f32x4 *)partial,
+                       pl.splits);
+    RCV_LAUNCH_CHECK();
+    return RCV_OK;
+}
+
+template <typename T, typename S> int launch_tile(const I8Product &p, const Plan &pl, void *ws, hipStream_t st)
 {
     static std::atomic<unsigned long long> ready{0};
     const int rc = allow_lds((const void *)k_i8_tile<T, S>, S::LDS, ready);
     if (rc != RCV_OK) return rc;
     const long long tm = (p.rows + S::BM - 1) / S::BM, tn = (p.Cout + S::BN - 1) / S::BN;
     if (tm * tn > 0x7fffffffLL) return RCV_E_TOO_LARGE;
-    hipLaunchKernelGGL((k_i8_tile<T, S>), dim3((unsigned)(tm * tn), 1, p.groups), dim3(64 * S::NW), S::LDS, st, p, (int)tm, (int)tn);
+    f32x4 *partial = S::SPLIT ? (f32x4 *)ws : nullptr;
+    hipLaunchKernelGGL((k_i8_tile<T, S>), dim3((unsigned)(tm * tn), pl.splits, p.groups), dim3(64 * S::NW), S::LDS, st, p, (int)tm, (int)tn, partial);
     RCV_LAUNCH_CHECK();
-    return RCV_OK;
+    return partial ? launch_finish<T, S::TAPS>(p, pl, partial, st) : RCV_OK;
 }
 
-// How a product runs.
-struct Plan {
-    enum Kind { TILE, DIRECT64, DIRECT16 } kind;
-    int splits;
-    size_t bytes;  // of partial sums
-};
-
-Plan plan_product(long long rows, int K, int Cout, int taps, int groups)
+template <typename T, int TAPS, int TT, int CT, int D> int launch_direct(const I8Product &p, const Plan &pl, void *ws, hipStream_t st)
 {
-    Plan pl{Plan::TILE, 1, 0};
-    const long long tiles = ((rows + 255) / 256) * ((Cout + 127) / 128) * groups;
-    if (tiles >= 128) return pl;
-    pl.kind = rows <= 16 ? Plan::DIRECT16 : Plan::DIRECT64;
-    const int edge = rows <= 16 ? 16 : 64;
-    const long long wgs = ((rows + edge - 1) / edge) * ((Cout + edge - 1) / edge) * groups;
-    const int steps = taps * ((K + 63) / 64);
-    while (wgs * pl.splits * 2 <= 512 && steps >= pl.splits * 2 * 8 * 4) pl.splits *= 2;  // (at least four steps a wave)
-    if (pl.splits > 1) pl.bytes = (size_t)pl.splits * groups * rows * ((Cout + 3) / 4) * 16;
-    return pl;
-}
-
-template <typename T, int TAPS, int TT, int CT> int launch_direct(const I8Product &p, const Plan &pl, void *ws, hipStream_t st)
-{
-    constexpr int NW = 8, D = TT == 1 ? 4 : 1, LDS = NW * TT * 16 * (CT * 16 + 4) * 4;
+    constexpr int NW = 8, LDS = NW * TT * 16 * (CT * 16 + 4) * 4;
     static std::atomic<unsigned long long> ready{0};
     if (LDS > 64 * 1024) {
         const int rc = allow_lds((const void *)k_i8_direct<T, TAPS, TT, CT, NW, D>, LDS, ready);
@@ -764,27 +847,30 @@ template <typename T, int TAPS, int TT, int CT> int launch_direct(const I8Produc
     hipLaunchKernelGGL((k_i8_direct<T, TAPS, TT, CT, NW, D>), dim3((unsigned)(tm * tn), pl.splits, p.groups), dim3(64 * NW), LDS, st, p, (int)tn,
                        partial);
     RCV_LAUNCH_CHECK();
-    if (partial) {
-        const long long quads = p.rows * ((p.Cout + 3) / 4);
-        hipLaunchKernelGGL((k_i8_finish<T, TAPS>), dim3((unsigned)((quads + 255) / 256), 1, p.groups), dim3(256), 0, st, p,
-                           (const f32x4 *)partial, pl.splits);
-        RCV_LAUNCH_CHECK();
-    }
-    return RCV_OK;
+    return partial ? launch_finish<T, TAPS>(p, pl, partial, st) : RCV_OK;
 }
 
 template <typename T, int TAPS> int launch_taps(const I8Product &p, const Plan &pl, void *ws, hipStream_t st)
 {
-    if (pl.kind == Plan::TILE) return launch_tile<T, TileShape<TAPS, 4, 2, 4, 4, 128, 3>>(p, st);
-    if (pl.kind == Plan::DIRECT16) return launch_direct<T, TAPS, 1, 1>(p, pl, ws, st);
-    return launch_direct<T, TAPS, 4, 4>(p, pl, ws, st);
+    if (pl.kind == Plan::DIRECT) {
+        if (p.rows <= 16) return launch_direct<T, TAPS, 1, 1, TAPS == 1 ? 4 : 2>(p, pl, ws, st);
+        if (p.rows <= 32) return launch_direct<T, TAPS, 2, 1, TAPS == 1 ? 4 : 2>(p, pl, ws, st);
+        return launch_direct<T, TAPS, 4, 1, 2>(p, pl, ws, st);
+    }
+    if constexpr (TAPS == 1) {
+        if (pl.kind == Plan::WIDE) return launch_tile<T, TileShape<1, 2, 4, 8, 4, 3, 2>>(p, pl, ws, st);
+        if (pl.splits > 1) return launch_tile<T, TileShape<1, 4, 2, 2, 4, 5, 4, true>>(p, pl, ws, st);
+        return launch_tile<T, TileShape<1, 4, 2, 2, 4, 3, 2>>(p, pl, ws, st);
+    } else {
+        if (pl.kind == Plan::TALL) return launch_tile<T, TileShape<9, 4, 2, 4, 4, 3, 3>>(p, pl, ws, st);
+        if (pl.kind == Plan::NARROW) return launch_tile<T, TileShape<9, 8, 1, 2, 4, 3, 3>>(p, pl, ws, st);
+        if (pl.splits > 1) return launch_tile<T, TileShape<9, 4, 2, 2, 4, 5, 4, true>>(p, pl, ws, st);
+        return launch_tile<T, TileShape<9, 4, 2, 2, 4, 5, 4>>(p, pl, ws, st);
+    }
 }
 
-template <typename T> int launch_product(I8Product p, void *ws, hipStream_t st)
+template <typename T> int launch_product(const I8Product &p, void *ws, hipStream_t st)
 {
-    const size_t four = 4 * sizeof(T);  // rows of output (and residual) that can be moved four channels at a time
-    p.vec = (uintptr_t)p.out % four == 0 && p.out_pitch % 4 == 0 && p.out_gs % 4 == 0 &&
-            (!p.residual || ((uintptr_t)p.residual % four == 0 && p.residual_pitch % 4 == 0 && p.residual_gs % 4 == 0));
     const Plan pl = plan_product(p.rows, p.K, p.Cout, p.taps, p.groups);
     return p.taps == 9 ? launch_taps<T, 9>(p, pl, ws, st) : launch_taps<T, 1>(p, pl, ws, st);
 }

@@ -14,7 +14,7 @@ struct I8Product {
     long long rows, code_pitch, residual_pitch, out_pitch;
     long long code_gs, weight_scale_gs, bias_gs, residual_gs, out_gs;  // (the token scales' group stride is code_gs as well)
     int K, kp, Cout, taps, H, W;
-    int relu, out_dtype, groups, vec;   // vec: set by the launch
+    int relu, out_dtype, groups;
     unsigned *range;                    // RCV_F16 engines: the sticky range-flag word, or null
 };
 

@@ -177,7 +177,8 @@ MATMUL = [(1, 1, 1), (1, 16, 5), (1, 4096, 300), (2, 131, 17), (3, 100, 33), (16
           (100, 2048, 96), (130, 130, 129), (256, 128, 128), (257, 384, 257), (300, 2048, 512), (515, 96, 40), (2049, 256, 200), (5000, 64, 8),
           (777, 1500, 333),
           # enough output tiles for the large-product kernel: many rows of few channels, few rows of many
-          (33000, 70, 40), (33023, 200, 9), (300, 150, 16500)]
+          (33000, 70, 40), (33023, 200, 9), (300, 150, 16500),
+          (12300, 1030, 1025)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
@@ -199,7 +200,7 @@ def test_matmul(m, k, n, dtype):
 CONV = [(1, 1, 1, 16, 1), (1, 1, 9, 64, 32), (2, 9, 1, 48, 24), (2, 5, 7, 33, 19), (1, 15, 20, 256, 96), (3, 37, 53, 96, 80), (1, 2, 2, 1, 1),
         (5, 8, 8, 128, 130), (2, 15, 20, 640, 64), (1, 61, 70, 64, 200),
         # enough output tiles for the large-product kernel
-        (9, 61, 70, 33, 24), (7, 47, 101, 130, 136), (33001, 1, 1, 20, 8), (1, 33000, 2, 16, 4)]
+        (9, 61, 70, 33, 24), (7, 47, 101, 130, 120), (7, 47, 101, 40, 136), (33001, 1, 1, 20, 8), (1, 33000, 2, 16, 4)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
