@@ -157,12 +157,6 @@ __global__ __launch_bounds__(1024) void k_i8_quantize_long(const T *x0, long lon
 }
 
 // A view of memory for buffer loads: what lies beyond `bytes` reads as zeros.
-__device__ __forceinline__ i32x4 descriptor(const int8_t *base, long long bytes)
-{
-    const unsigned long long b = (unsigned long long)base;
-    const long long n = bytes < 0 ? 0 : bytes > 0x7fffffffLL ? 0x7fffffffLL : bytes;
-    return i32x4{(int)(unsigned)b, (int)((unsigned)(b >> 32) & 0xffffu), (int)n, 0x00020000};
-}
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t view(const int8_t *base, long long bytes)
 {
     return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, bytes < 0 ? 0 : bytes > 0x7fffffffLL ? 0x7fffffff : (int)bytes, 0x00020000);
@@ -431,7 +425,7 @@ template <int TAPS_, int WT_, int WC_, int TT_, int CT_, int NA_, int NB_, bool 
     static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;      // pieces (8 rows) of a wave per step
     static constexpr int A_BYTES = BM * KB, B_BYTES = BN * KB, B_RING = NA * A_BYTES, TABLE = B_RING + NB * B_BYTES;
     static constexpr int LDS = TABLE + (TAPS == 9 ? 9 * BM * 4 : 0);
-    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && LDS <= 160 * 1024 && NA >= 3 && NB >= 2 && NB <= NA, "tile plan");
+    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && LDS <= 160 * 1024 && NA >= 3 && NB >= 2 && NB <= NA && BM <= 64 * NW, "tile plan");
     // Pieces in order of issue, per step kt: the tokens of step kt + NA - 1 in its first half, the weights of step kt + NB in its second.
     // Half-way through step kt everything of step kt + 1 has to be there: what may still be on its way was issued later.
     static constexpr int LATE = NB == NA ? (NA - 2) * (PA + PB) : (NB - 2) * (PA + PB) + PA;
@@ -471,11 +465,9 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_i8_tile(const I8Product p, in
     const long long m0 = (long long)mt * BM;
     const int left = (int)min((long long)BM, p.rows - m0);
     const int8_t *codes = p.codes + (long long)g * p.code_gs * p.code_pitch;
-    const int8_t *codes_end = codes + (p.rows - 1) * p.code_pitch + ((p.K + 15) & ~15);
     const float *cs = p.code_scales + (long long)g * p.code_gs;
     const int wrow = TAPS * p.kp;
     const int8_t *wts = p.weights + ((long long)g * p.Cout + n0) * wrow;
-    const long long wbytes = (long long)(p.Cout - n0) * wrow;
 
     // which of the nine taps of a token lie inside its image
     const int W = p.W, H = p.H;
@@ -550,14 +542,34 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_i8_tile(const I8Product p, in
         return false;
     };
     Walk ia{tap0, klo, 0}, ib{tap0, klo, 0};
-    i32x4 ra, rb;
     unsigned a_lds = lds0 + wave * PA * 1024, b_lds = lds0 + S::B_RING + wave * PB * 1024;
     const unsigned a_last = a_lds + (S::NA - 1) * S::A_BYTES, b_last = b_lds + (S::NB - 1) * S::B_BYTES;
-    auto a_tap = [&]() {
-        const int8_t *a = codes + (m0 + (TAPS == 9 ? (long long)(ia.tap / 3 - 1) * W + (ia.tap % 3 - 1) : 0)) * pitch;
-        ra = descriptor(a, codes_end - a);
+    // The descriptors of a tap, in few scalar instructions (every wave runs them, all matrix units wait): the tokens move by `shift` rows, and
+    // the view ends with the tile's or the tensor's last row, whichever comes first.
+    i32x4 ra, rb;
+    const long long next_col = pitch, next_row = (long long)(W - 2) * pitch;
+    const int below = (int)min(p.rows - m0, 1LL << 30), last_row = (int)pitch - ((p.K + 15) & ~15);
+    long long a_at = (long long)(codes + (m0 + (TAPS == 9 ? (long long)(tap0 / 3 - 1) * W + (tap0 % 3 - 1) : 0)) * pitch);
+    int a_col = tap0 % 3, shift = TAPS == 9 ? (tap0 / 3 - 1) * W + a_col - 1 : 0;
+    long long b_at = (long long)(wts + (long long)tap0 * p.kp);
+    int b_bytes = min(p.Cout - n0, BN) * wrow - tap0 * p.kp;
+    auto a_view = [&]() {
+        const int rows = min(below - shift, BM);
+        ra = i32x4{(int)a_at, (int)(a_at >> 32) & 0xffff, rows > 0 ? rows * (int)pitch - last_row : 0, 0x00020000};
     };
-    auto b_tap = [&]() { rb = descriptor(wts + (long long)ib.tap * p.kp, wbytes - (long long)ib.tap * p.kp); };
+    auto b_view = [&]() { rb = i32x4{(int)b_at, (int)(b_at >> 32) & 0xffff, b_bytes, 0x00020000}; };
+    auto a_tap = [&]() {
+        const bool wrap = ++a_col == 3;
+        a_col = wrap ? 0 : a_col;
+        a_at += wrap ? next_row : next_col;
+        shift += wrap ? W - 2 : 1;
+        a_view();
+    };
+    auto b_tap = [&]() {
+        b_at += p.kp;
+        b_bytes -= p.kp;
+        b_view();
+    };
     auto a_piece = [&](auto cc) {
         constexpr int c = decltype(cc)::value;
         int v = aoff[c];
@@ -577,8 +589,8 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_i8_tile(const I8Product p, in
         if (step(ib)) b_tap();
     };
 
-    a_tap();
-    b_tap();
+    a_view();
+    b_view();
     asm volatile("s_nop 4");  // (scalars that came through vector registers, before the first piece reads them)
     for (int s = 0; s < S::NA - 1; s++) {  // tokens of steps 0 .. NA - 2 and weights of steps 0 .. NB - 1 in the order of the loop
         for_each<0, PA>(a_piece);
@@ -595,11 +607,16 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_i8_tile(const I8Product p, in
 
     float *sa_tab = (float *)(smem + S::TABLE);  // [9][BM]: the scale under which a token's tap enters, 0 outside the image
     if constexpr (TAPS == 9) {
-        for (int row = tid; row < BM; row += 64 * S::NW) {
-            const unsigned ok = taps_inside(row);
+        // (nine loads in flight: outside the image the offset is out of range and the load gives 0)
+        const __amdgpu_buffer_rsrc_t view_s = view((const int8_t *)(cs + (m0 - W - 1)), (p.rows - m0 + W + 1) * 4);
+        if (tid < BM) {
+            const unsigned ok = taps_inside(tid);
+            float v[9];
 #pragma unroll
             for (int t = 0; t < 9; t++)
-                sa_tab[t * BM + row] = (ok >> t) & 1u ? cs[m0 + row + (long long)(t / 3 - 1) * W + (t % 3 - 1)] : 0.f;
+                v[t] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(view_s, (ok >> t) & 1u ? (tid + (t / 3) * W + t % 3) * 4 : OOB, 0, 0));
+#pragma unroll
+            for (int t = 0; t < 9; t++) sa_tab[t * BM + tid] = v[t];
         }
     }
 
