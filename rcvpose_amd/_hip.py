@@ -137,8 +137,8 @@ SYMBOLS = {
     "rcv_i8_quantize_tokens": (_i, [_vp, ctypes.c_longlong, _i, _vp, ctypes.c_longlong, _i, _i, ctypes.c_longlong, _vp, ctypes.c_longlong, _vp, _vp]),
     "rcv_i8_matmul_workspace_bytes": (_sz, [ctypes.c_longlong, _i, _i]),
     "rcv_i8_conv3x3_workspace_bytes": (_sz, [ctypes.c_longlong, _i, _i]),
-    "rcv_i8_matmul": (_i, [ctypes.POINTER(I8Args), _vp, _sz, _vp]),
-    "rcv_i8_conv3x3": (_i, [ctypes.POINTER(I8Args), _vp, _sz, _vp]),
+    "rcv_i8_matmul": (_i, [_vp, _vp, _sz, _vp]),
+    "rcv_i8_conv3x3": (_i, [_vp, _vp, _sz, _vp]),
     "rcv_icp_point_to_point": (_i, [_vp, _i, _vp, _i, _d, ctypes.POINTER(_d), _d, _d, _i, _vp, _vp, _sz, _vp]),
 }
 
@@ -219,10 +219,3 @@ def current_stream():
     import torch
 
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
-
-
-def raw_stream(index):
-    """hipStream_t of device `index`'s current stream, as an integer (current_stream without the Stream object: 4 us less per call)."""
-    import torch
-
-    return torch._C._cuda_getCurrentRawStream(index)

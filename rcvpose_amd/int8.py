@@ -10,6 +10,7 @@ these kernels.  Inference only; there is no CPU fallback.  Results do not depend
 have a fixed order.  The reference has no counterpart (its forward is fp32, models/fcnresnet.py:121-191).
 """
 import ctypes
+import struct
 
 import torch
 
@@ -18,6 +19,8 @@ from . import _hip
 KP = 128  # weight rows are zero-padded to a multiple of this many codes per tap (include/rcvpose_hip.h)
 MAX_CHANNELS = 131071
 _ARGS_BYTES = ctypes.sizeof(_hip.I8Args)
+_pack_args = struct.Struct("@Ii7P4q6i").pack  # struct rcv_i8_args (a ctypes structure takes a microsecond longer to fill)
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _DTYPES = {torch.float32: _hip.RCV_F32, torch.bfloat16: _hip.RCV_BF16, torch.float16: _hip.RCV_F16}
 
 
@@ -93,26 +96,23 @@ def _rows(t):
     return t, t.numel() // c, c
 
 
-def _check_device(dev, *others):
-    """Every tensor of a call lives on `dev`."""
-    for t in others:
-        if t is not None and t.device != dev:
-            if not t.is_cuda:
-                _no_cpu()
-            raise ValueError("all tensors of a call must be on one device")
+def _elsewhere(t):
+    """The error for a tensor that is not where the call's first tensor is."""
+    if not t.is_cuda:
+        _hip.lib()  # (raises first where no GPU is visible)
+        raise RuntimeError("rcvpose_amd runs on MI355X only: move the tensors to 'cuda' (no CPU fallback)")
+    raise ValueError("all tensors of a call must be on one device")
 
 
-def _no_cpu():
-    _hip.lib()  # (raises first where no GPU is visible)
-    raise RuntimeError("rcvpose_amd runs on MI355X only: move the tensors to 'cuda' (no CPU fallback)")
-
-
-def _on_device(dev, call):
-    """call() with `dev` as the current device (the launch goes to dev's current stream)."""
-    if torch.cuda.current_device() == dev.index:
-        return call()
-    with torch.cuda.device(dev):
-        return call()
+def _launch(index, name, fn, *args):
+    """fn(*args, stream) with device `index` current, on that device's current stream."""
+    if _current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _hip.check(rc, name)
 
 
 def quantize_tokens(x, x1=None):
@@ -132,23 +132,22 @@ def quantize_tokens(x, x1=None):
     c = c0 + c1
     if c > MAX_CHANNELS:
         raise ValueError("a token has at most %d channels" % MAX_CHANNELS)
-    if not x.is_cuda:
-        _no_cpu()
-    dev = x.device
-    _check_device(dev, x1)
+    index = x.get_device()
+    if index < 0:
+        _elsewhere(x)
     x, rows, pitch0 = _rows(x)
     pitch1, x1_ptr = 0, None
     if x1 is not None:
+        if x1.get_device() != index:
+            _elsewhere(x1)
         x1, _, pitch1 = _rows(x1)
         x1_ptr = x1.data_ptr()
     pitch = (c + 15) // 16 * 16
-    codes = torch.empty(shape[:-1] + (pitch,), dtype=torch.int8, device=dev)
-    scales = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+    lead = shape[:-1]
+    codes, scales = x.new_empty(lead + (pitch,), dtype=torch.int8), x.new_empty(lead, dtype=torch.float32)
     if rows:
-        rc = _on_device(dev, lambda: L.rcv_i8_quantize_tokens(x.data_ptr(), pitch0, c0, x1_ptr, pitch1, c1, dtype, rows, codes.data_ptr(), pitch,
-                                                              scales.data_ptr(), _hip.raw_stream(dev.index)))
-        if rc:
-            _hip.check(rc, "rcv_i8_quantize_tokens")
+        _launch(index, "rcv_i8_quantize_tokens", L.rcv_i8_quantize_tokens, x.data_ptr(), pitch0, c0, x1_ptr, pitch1, c1, dtype, rows,
+                codes.data_ptr(), pitch, scales.data_ptr())
     return codes if pitch == c else codes[..., :c], scales
 
 
@@ -163,12 +162,14 @@ def _product(name, codes, scales, weight, bias, residual, relu, dtype, height, w
     out_type = _DTYPES.get(dtype)
     if out_type is None:
         raise ValueError("output type must be torch.float32, torch.bfloat16 or torch.float16")
-    if not codes.is_cuda:
-        _no_cpu()
-    dev = codes.device
-    _check_device(dev, scales, weight.codes, weight.scales, bias, residual)
-    out = torch.empty(lead + (n,), dtype=dtype, device=dev)
-    bias_ptr, res_ptr, res_pitch = None, None, 0
+    index = codes.get_device()
+    if index < 0:
+        _elsewhere(codes)
+    for t in (scales, weight.codes, weight.scales, bias, residual):
+        if t is not None and t.get_device() != index:
+            _elsewhere(t)
+    out = codes.new_empty(lead + (n,), dtype=dtype)
+    bias_ptr = res_ptr = res_pitch = 0
     if bias is not None:
         if bias.dtype != torch.float32 or bias.shape != (n,):
             raise ValueError("bias must be float32 [%d]" % n)
@@ -182,22 +183,18 @@ def _product(name, codes, scales, weight, bias, residual, relu, dtype, height, w
     codes, rows, pitch = _rows(codes)
     if rows == 0:
         return out
-    need = (k + 15) // 16 * 16
+    ptr, need = codes.data_ptr(), (k + 15) // 16 * 16
     if rows == 1:  # (one row has no pitch of its own)
         pitch = need
-    codes_ptr = codes.data_ptr()
-    if pitch % 16 or codes_ptr % 16 or codes.untyped_storage().nbytes() - codes.storage_offset() < (rows - 1) * pitch + need:
+    if pitch % 16 or ptr % 16 or (need != k and codes.untyped_storage().nbytes() - codes.storage_offset() < (rows - 1) * pitch + need):
         raise ValueError("token rows must start 16 bytes aligned and be readable up to a multiple of 16 channels: "
                          "take the codes as quantize_tokens lays them out")
     scales = scales.contiguous()
-    args = _hip.I8Args(_ARGS_BYTES, out_type, codes_ptr, scales.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(), bias_ptr, res_ptr,
-                       out.data_ptr(), rows, pitch, res_pitch, n, k, n, height, width, 1 if relu else 0, 0)
-    call, workspace_bytes = getattr(L, name), getattr(L, name + "_workspace_bytes")
-    nbytes = workspace_bytes(rows, k, n)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    rc = _on_device(dev, lambda: call(ctypes.byref(args), None if ws is None else ws.data_ptr(), nbytes, _hip.raw_stream(dev.index)))
-    if rc:
-        _hip.check(rc, name)
+    args = _pack_args(_ARGS_BYTES, out_type, ptr, scales.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(), bias_ptr, res_ptr,
+                      out.data_ptr(), rows, pitch, res_pitch, n, k, n, height, width, 1 if relu else 0, 0)
+    nbytes = getattr(L, name + "_workspace_bytes")(rows, k, n)
+    ws = codes.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _launch(index, name, getattr(L, name), args, None if ws is None else ws.data_ptr(), nbytes)
     return out
 
 
