@@ -51,6 +51,7 @@ def parse(argv=None):
                     help="FCN arithmetic: f16x3 (default; fp16 hi/lo pairs, 3 MFMAs per product: the fast mode within north_star's "
                          "1e-4 map tolerance), fp32 (v_mfma_f32_16x16x4_f32), bf16 / fp16 (throughput modes outside the tolerance)")
     ap.add_argument("--overlap", action="store_true", help="FCN of batch s+1 and voting of batch s on two HIP streams")
+    ap.add_argument("--int8", action="store_true", help="bf16 / fp16 only: the decoder's wide 3x3 convolutions on 8-bit integers (engine option 16; off by default)")
     ap.add_argument("--q6", action="store_true", help="f16x3 only: fp6 cross terms in the stride-1 3x3 convolutions of layers 2-4 (engine option 11; "
                                                       "-3 % forward time for 2-3x the map error, still inside the 1e-4 tolerance: off by default)")
     ap.add_argument("--no-cpu-baseline", action="store_true")
@@ -388,7 +389,8 @@ def main(argv=None):
     shapes = json.load(open(os.path.join(ROOT, "tests", "golden", "fcn_state_dict_keys.json")))
     sds = [{k: torch.from_numpy(v) for k, v in synthetic_weights.make_state_dict_numpy(shapes, seed=s).items()}
            for s in range(G)]
-    pipe = FramePipeline(sds, H, W, dtype=args.dtype, frames_per_step=B, overlap=args.overlap, q6=args.q6 and args.dtype == "f16x3")
+    pipe = FramePipeline(sds, H, W, dtype=args.dtype, frames_per_step=B, overlap=args.overlap, q6=args.q6 and args.dtype == "f16x3",
+                         int8=args.int8 and args.dtype in ("bf16", "fp16"))
 
     # frames are sharded over ranks: global frame f -> rank f % world; local frame i of rank r is the
     # synthetic frame r + world * i.  A pool of distinct frames per rank is cycled, resident in HBM before the timed region.
@@ -603,7 +605,7 @@ def main(argv=None):
                                       "the LDS shell rasteriser (k_vote) is its fallback and is timed in extras.rasteriser_engine_frames_per_s",
                        "frames_per_step_per_gpu": B, "distinct_frames_cycled": pool,
                        "weights": "random (seeded He), ideal maps injected after the forward",
-                       "overlap": bool(args.overlap), "q6_cross_terms": bool(args.q6 and args.dtype == "f16x3"), "parallelism": "frames sharded f%%%d, 1 RCCL all_gather/step" % world},
+                       "overlap": bool(args.overlap), "q6_cross_terms": bool(args.q6 and args.dtype == "f16x3"), "int8_decoder": bool(args.int8 and args.dtype in ("bf16", "fp16")), "parallelism": "frames sharded f%%%d, 1 RCCL all_gather/step" % world},
             "roofline": {"bound": "mfma", "achieved": achieved, "peak": peak, "unit": "TFLOP/s", "frac": achieved / peak,
                          "traffic": traffic, "traffic_unit": "HBM bytes per step (all conv launches)", "traffic_source": traffic_src,
                          "algorithmic_flop_per_step": conv_flop_step,

@@ -45,10 +45,10 @@ typedef enum rcv_status {
 
 const char *rcv_strerror(int status);
 /* ABI version of this header: bumped whenever a struct layout, an entry point's signature or a documented behaviour changes
- * (600 = round 6: rcv_op grew wq_off (88 bytes), rcv_fcn_range_status takes a stream, rcv_abi_check, RCV_SEAM_COUNT_NONFINITE).
+ * (700: rcv_i8_*, rcv_op::wq_off of the 16-bit engines, engine option 16; 600: rcv_op grew wq_off (88 bytes), rcv_fcn_range_status takes a stream, rcv_abi_check, RCV_SEAM_COUNT_NONFINITE).
  * rcv_version() returns the library's value; a binding compiled against another header must refuse to run (an ops array with
  * the wrong stride would be read as a garbage program): call rcv_abi_check once after loading the library. */
-#define RCV_ABI_VERSION 600
+#define RCV_ABI_VERSION 700
 int rcv_version(void);
 /* RCV_OK iff the caller's header matches the library: version == rcv_version() and the struct sizes the caller compiled
  * (sizeof(rcv_op), sizeof(rcv_acc_result), sizeof(rcv_strided), sizeof(rcv_icp_result)) equal the library's; RCV_E_INVALID otherwise. */
@@ -313,7 +313,10 @@ typedef struct rcv_op {
     int64_t wq_off;          /* RCV_F16X3: element offset of a SECOND copy of this op's weights, or 0 = none.  For a 3x3 / stride-1 op:
                               * the q6 row layout (engine option 11, below).  For the conv7 op of the tail (the 3x3 behind the last
                               * upsampling): the parity-composed weights [G][4 * cout][3][3][cin] of engine option 13, whose
-                              * [bias x 4 | scale] records sit behind the first copy's in the bias blob */
+                              * [bias x 4 | scale] records sit behind the first copy's in the bias blob.
+                              * RCV_BF16 / RCV_F16: element offset (2-byte elements, 16-byte aligned) of an int8 copy of a stride-1 1x1 or 3x3
+                              * op's weights, or 0 = none: [G][cout][k*k][channels rounded up to a multiple of 128] codes as rcv_i8_matmul /
+                              * rcv_i8_conv3x3 take them, and behind the op's biases [G][cout] the weight scales [G][cout] (engine option 16) */
 } rcv_op;
 
 typedef struct rcv_fcn rcv_fcn; /* opaque engine handle */
@@ -417,7 +420,11 @@ int rcv_fcn_set_profiling(rcv_fcn *h, int enable);
  * once, as a residual) in a 3-byte form (sign / 5-bit exponent / 18-bit mantissa, 96 instead of 128 bytes per 32-channel group): maps within
  * 6e-6 of the [hi | lo] form, 20 % fewer bytes, and SLOWER (9.5 against 7.2 ms per forward of 53 x 3: the encode / decode instructions).
  * key 15 (default 0 -- a measured experiment, r06; RCV_F16X3): the 128-wide chain kernel as four-wave workgroups (three per CU): bit-identical,
- * 7.9 against 7.3 ms. */
+ * 7.9 against 7.3 ms.
+ * key 16 (default 1, RCV_BF16 / RCV_F16): 8-bit integer arithmetic for the ops whose wq_off names an int8 copy of their weights: the op's
+ * source pixels are quantised (rcv_i8_quantize_tokens, one scale per pixel over the concatenated channels) into scratch behind the
+ * activation slots, then multiplied as integers (rcv_i8_matmul / rcv_i8_conv3x3).  The key only ENABLES the form, an op takes it when it has
+ * the copy, and such an op joins none of the fused kernels.  0: the 16-bit kernels (maps as without the copies). */
 int rcv_fcn_set_option(rcv_fcn *h, int key, int value);
 int rcv_fcn_get_profile(rcv_fcn *h, double *conv_ms, double *other_ms, double *conv_flop);
 /* Per-op device times (ms) of the last profiled forward; ms_out has room for n_ops doubles. */

@@ -523,7 +523,7 @@ def estimate_6d_pose_lm(opts, return_details=False):
             import gc
 
             dtype_ = getattr(opts, 'dtype', 'f16x3')
-            fcn = FcnEngine(sds, H, W, dtype=dtype_)
+            fcn = FcnEngine(sds, H, W, dtype=dtype_, int8=getattr(opts, 'int8', False))
             pipe = None
             while pipe is None:
                 n_batches = (len(todo) + n_step - 1) // n_step
@@ -746,7 +746,7 @@ def estimate_6d_pose_lmo(opts, return_details=False):
                 estimated_kpts, statuses = np.zeros((3, 3)), []
                 if opts.using_ckpts:
                     if pipe is None:
-                        pipe = FramePipeline(sds, H, W, dtype=getattr(opts, 'dtype', 'f16x3'), frames_per_step=1)
+                        pipe = FramePipeline(sds, H, W, dtype=getattr(opts, 'dtype', 'f16x3'), frames_per_step=1, int8=getattr(opts, 'int8', False))
                         pipe.set_stage_timing(True)
                         pipe.seg_threshold = seg_thr
                     rgb = np.array(Image.open(jpgPath + filename).convert('RGB'), dtype=np.uint8)
@@ -900,7 +900,7 @@ def estimate_6d_pose_ycb(opts, return_details=False):
             H, W = depth_map1.shape
             depth_dev = _depth_to_u16(depth_map1, "cuda")
             if pipe is None:
-                pipe = FramePipeline(sds, H, W, dtype=getattr(opts, 'dtype', 'f16x3'), frames_per_step=1)
+                pipe = FramePipeline(sds, H, W, dtype=getattr(opts, 'dtype', 'f16x3'), frames_per_step=1, int8=getattr(opts, 'int8', False))
                 pipe.set_stage_timing(True)
                 ws = AccWorkspace(H * W)
             pipe._mark("begin_net")

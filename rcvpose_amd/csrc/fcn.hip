@@ -33,6 +33,7 @@
 #include <vector>
 
 #include "common.hpp"
+#include "int8.hpp"
 
 namespace rcv {
 namespace {
@@ -5111,6 +5112,7 @@ struct rcv_fcn {
     int use_splitk = 0;       // latency option (12): split-K in k_conv_lat + k_splitk_finish for launches with few tiles (one or a few frames)
     float *splitk_ws = nullptr;  // ... its partial sums (allocated when the option is switched on, never on the hot path)
     size_t splitk_bytes = 0;
+    int use_int8 = 1;         // 16-bit engines (16): 8-bit integer arithmetic for the ops whose weights come with an int8 copy (rcv_op::wq_off)
     int use_q6 = 1;           // split engine: fp6 cross terms (k_conv_halo<.., true>) for the ops whose weights come with a q6 copy (rcv_op::wq_off)
     // range guard of the half-precision engines: one sticky flag word on the device (kernels OR bits into it), mirrored into
     // pinned host memory by a 4-byte copy at the end of every forward
@@ -5132,6 +5134,72 @@ void slot_offsets(const rcv_fcn *h, int B, std::vector<size_t> &off, size_t &tot
         o += align_up((size_t)h->slot_elems[i] * (size_t)h->groups * (size_t)B * esize(h->dtype), 256);
     }
     total = o;
+}
+
+// ---- 8-bit integer arithmetic (16-bit engines): an op whose wq_off names an int8 copy of its weights quantises its source pixels
+// [c0 | c1] into the scratch behind the slots -- codes, then one scale per pixel -- and runs as rcv_i8_matmul / rcv_i8_conv3x3 do.
+bool i8_op(const rcv_fcn *h, const rcv_op &o)
+{
+    return (h->dtype == RCV_BF16 || h->dtype == RCV_F16) && o.kind == RCV_OP_CONV && o.wq_off > 0;
+}
+struct I8Scratch {
+    size_t scales, partial, bytes;  // offsets of the scales and of the partial sums behind the codes
+};
+I8Scratch i8_scratch(const rcv_fcn *h, const rcv_op &o, int B)
+{
+    const long long rows = (long long)B * o.hin * o.win;
+    const int C = o.c0 + (o.src1 >= 0 ? o.c1 : 0);
+    I8Scratch s;
+    s.scales = align_up((size_t)rows * h->groups * align_up((size_t)C, 16), 256);
+    s.partial = align_up(s.scales + (size_t)rows * h->groups * 4, 256);
+    s.bytes = align_up(s.partial + i8_product_workspace(rows, C, o.cout, o.ksize * o.ksize, h->groups), 256);
+    return s;
+}
+size_t i8_scratch_bytes(const rcv_fcn *h, int B)
+{
+    size_t most = 0;
+    for (const rcv_op &o : h->ops)
+        if (i8_op(h, o)) most = std::max(most, i8_scratch(h, o, B).bytes);
+    return most;
+}
+int run_int8(rcv_fcn *h, const rcv_op &o, int B, char *ws, const std::vector<size_t> &off, char *scratch, hipStream_t st)
+{
+    const long long rows = (long long)B * o.hin * o.win;
+    const int c1 = o.src1 >= 0 ? o.c1 : 0, C = o.c0 + c1;
+    const I8Scratch s = i8_scratch(h, o, B);
+    auto gs = [&](int slot) -> long long { return (long long)h->slot_elems[slot] * B; };
+    I8Product p{};
+    p.code_pitch = (long long)align_up((size_t)C, 16);
+    int8_t *codes = (int8_t *)scratch;
+    float *scales = (float *)(scratch + s.scales);
+    // one launch for all groups where their pixels follow one another
+    const bool joined = gs(o.src0) == rows * o.c0 && (o.src1 < 0 || gs(o.src1) == rows * c1);
+    for (int g = 0; g < (joined ? 1 : h->groups); g++) {
+        const int rc = i8_quantize(ws + off[o.src0] + 2 * g * gs(o.src0), o.c0, o.c0, o.src1 >= 0 ? ws + off[o.src1] + 2 * g * gs(o.src1) : nullptr,
+                                   c1, c1, h->dtype, joined ? rows * h->groups : rows, codes + g * rows * p.code_pitch, p.code_pitch,
+                                   scales + g * rows, st);
+        if (rc != RCV_OK) return rc;
+    }
+    p.codes = codes;
+    p.code_scales = scales;
+    p.code_gs = rows;
+    p.weights = (const int8_t *)h->weights + 2 * o.wq_off;
+    p.bias = h->bias + o.b_off;
+    p.bias_gs = o.cout;
+    p.weight_scales = p.bias + (long long)h->groups * o.cout;
+    p.weight_scale_gs = o.cout;
+    if (o.res >= 0) {
+        p.residual = ws + off[o.res];
+        p.residual_gs = gs(o.res);
+        p.residual_pitch = o.cout;
+    }
+    p.out = ws + off[o.dst];
+    p.out_gs = gs(o.dst);
+    p.out_pitch = o.cout;
+    p.rows = rows;
+    p.K = C; p.kp = i8_kp(C); p.Cout = o.cout; p.taps = o.ksize * o.ksize; p.H = o.hin; p.W = o.win;
+    p.relu = o.relu; p.out_dtype = h->dtype; p.groups = h->groups; p.range = h->range_dev;
+    return i8_product(p, scratch + s.partial, s.bytes - s.partial, st);
 }
 
 template <typename T, int BM, int BN>
@@ -5519,10 +5587,18 @@ int forward_impl(rcv_fcn *h, const float *x, int B, float *seg, float *radial, c
         return reader;
     };
     for (size_t i = 0; i < h->ops.size(); i++) {
+        if (sizeof(T) == 2 && !kX3 && h->use_int8 && i8_op(h, h->ops[i])) {
+            if (h->profiling) RCV_HIP_CHECK(hipEventRecord(h->events[2 * i], st));
+            const int rc = run_int8(h, h->ops[i], B, ws, off, ws + total, st);
+            if (rc != RCV_OK) return rc;
+            if (h->profiling) RCV_HIP_CHECK(hipEventRecord(h->events[2 * i + 1], st));
+            continue;
+        }
+        auto int8_at = [&](size_t k) { return !kX3 && h->use_int8 && k < h->ops.size() && i8_op(h, h->ops[k]); };  // (such an op joins no fused kernel)
         if constexpr (sizeof(T) == 2) {
             // 3x3 (-> 256 channels, ReLU) followed by the 1x1 expand to 1024 channels with residual and ReLU: the second
             // half of a layer-3 bottleneck block as one kernel (option 4)
-            if (!kX3 && h->use_block && i + 1 < h->ops.size() && h->ops[i].kind == RCV_OP_CONV && h->ops[i + 1].kind == RCV_OP_CONV &&
+            if (!kX3 && h->use_block && i + 1 < h->ops.size() && h->ops[i].kind == RCV_OP_CONV && h->ops[i + 1].kind == RCV_OP_CONV && !int8_at(i + 1) &&
                 (long long)h->slot_elems[h->ops[i + 1].dst] * B * 2 < 0x7fffffffLL) {  // (the widest tensor it touches; 32-bit DMA offsets)
                 const rcv_op &a = h->ops[i], &b = h->ops[i + 1];
                 const long long M = (long long)B * a.hout * a.wout;
@@ -5553,7 +5629,7 @@ int forward_impl(rcv_fcn *h, const float *x, int B, float *seg, float *radial, c
                     q.range = h->range_dev;
                     // the next block's 1x1 reduce (1024 -> 256, ReLU) reads exactly the tile this kernel produces: chained in
                     bool chain = false;
-                    if (h->use_chain && i + 2 < h->ops.size() && h->ops[i + 2].kind == RCV_OP_CONV) {
+                    if (h->use_chain && i + 2 < h->ops.size() && h->ops[i + 2].kind == RCV_OP_CONV && !int8_at(i + 2)) {
                         const rcv_op &c = h->ops[i + 2];
                         // (its output must not share a slot with anything the kernel still reads: other tiles are in flight)
                         chain = c.ksize == 1 && c.stride == 1 && c.pad == 0 && c.c0 == 4 * cmid && c.cout == cmid && c.src0 == b.dst &&
@@ -5638,7 +5714,7 @@ int forward_impl(rcv_fcn *h, const float *x, int B, float *seg, float *radial, c
                 }
             }
             // upsample x2 -> conv7 (3x3, 64 -> 32, ReLU) -> head (1x1, 32 -> 2): one fused kernel (option 3)
-            if (h->use_tail && i + 2 < h->ops.size() + 0 && h->ops[i].kind == RCV_OP_UPSAMPLE2 && h->ops[i + 1].kind == RCV_OP_CONV &&
+            if (h->use_tail && i + 2 < h->ops.size() + 0 && h->ops[i].kind == RCV_OP_UPSAMPLE2 && h->ops[i + 1].kind == RCV_OP_CONV && !int8_at(i + 1) &&
                 h->ops[i + 2].kind == RCV_OP_HEAD) {
                 const rcv_op &u = h->ops[i], &c = h->ops[i + 1], &d = h->ops[i + 2];
                 if (u.c0 == 64 && c.src0 == u.dst && c.src1 < 0 && c.res < 0 && c.c0 == 64 && c.cout == 32 && c.ksize == 3 &&
@@ -5824,6 +5900,17 @@ int rcv_fcn_create(const rcv_op *ops, int n_ops, int n_slots, const int64_t *slo
             if (!in_ok || !out_ok) return RCV_E_UNSUPPORTED;
         }
     }
+    if (dtype == RCV_BF16 || dtype == RCV_F16) {
+        // ops with an int8 copy of their weights: the shapes the integer kernels run, 16-byte aligned rows
+        for (int i = 0; i < n_ops; i++) {
+            const rcv_op &o = ops[i];
+            if (o.kind != RCV_OP_CONV || o.wq_off <= 0) continue;
+            const bool shape = (o.ksize == 1 && o.pad == 0) || (o.ksize == 3 && o.pad == 1);
+            if (!shape || o.stride != 1 || o.hin != o.hout || o.win != o.wout || o.win > (1 << 16) || o.c0 + (o.src1 >= 0 ? o.c1 : 0) > 131071)
+                return RCV_E_UNSUPPORTED;
+            if (o.src0 < 0 || o.dst < 0 || ((uintptr_t)weights_dev + 2 * (uintptr_t)o.wq_off) % 16) return RCV_E_INVALID;
+        }
+    }
     rcv_fcn *h = new rcv_fcn();
     if (dtype == RCV_F16 || dtype == RCV_F16X3) {  // the range guard's flag word and its pinned mirror (not on the hot path)
         hipError_t e = hipMalloc((void **)&h->range_dev, 256);
@@ -5880,7 +5967,7 @@ size_t rcv_fcn_workspace_bytes(const rcv_fcn *h, int B)
     std::vector<size_t> off;
     size_t total;
     slot_offsets(h, B, off, total);
-    return total;
+    return total + i8_scratch_bytes(h, B);
 }
 
 int rcv_fcn_forward(rcv_fcn *h, const float *x_dev, int B, float *seg_dev, float *radial_dev, void *ws, size_t ws_bytes,
@@ -5971,6 +6058,7 @@ int rcv_fcn_set_option(rcv_fcn *h, int key, int value)
     if (key == 13) { h->use_tailc = value; return RCV_OK; }
     if (key == 14) { h->use_t3 = value; return RCV_OK; }
     if (key == 15) { h->use_c2w4 = value; return RCV_OK; }
+    if (key == 16) { h->use_int8 = value != 0; return RCV_OK; }
     if (key == 12) {
         if (value && !h->splitk_ws) {
             const size_t bytes = (size_t)48 << 20;  // the largest split launch of the FCN programs at up to 3 networks x 1 frame needs 11 MB

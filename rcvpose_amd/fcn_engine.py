@@ -342,6 +342,19 @@ def q6_wanted(spec, op, pattern=Q6_DEFAULT):
             op["cout"] % 128 == 0 and re.fullmatch(pattern, spec["conv"]) is not None)
 
 
+INT8_DEFAULT = r"conv6|conv_up[543]\.0"
+
+
+def int8_wanted(spec, op, pattern=INT8_DEFAULT):
+    """The ops that get an int8 copy of their weights (8-bit integer products, engine option 16): stride-1 1x1 and 3x3 convolutions whose
+    name matches.  The default is the decoder's wide 3x3 convolutions: long sums, where the integer rate pays for the quantisation of the
+    source, and no fused 16-bit kernel that they would leave."""
+    import re
+
+    return (op["kind"] == _hip.OP_CONV and op["stride"] == 1 and (op["ksize"], op["pad"]) in ((1, 0), (3, 1)) and
+            re.fullmatch(pattern, spec["conv"]) is not None)
+
+
 # bilinear x2 (align_corners=False) seen from the 3x3 convolution that follows it: the high-resolution tap t - 1 (t = 0, 1, 2) of output
 # row 2i + p reads low-resolution rows i - 1, i, i + 1 with these weights (row p, then t, then k).  out[2i] = .25 in[i-1] + .75 in[i],
 # out[2i+1] = .75 in[i] + .25 in[i+1] (reference models/fcnresnet.py:93,177: nn.Upsample(scale_factor=2, mode='bilinear'))
@@ -377,9 +390,11 @@ def tail_composed_wanted(builder, i):
             c["c0"] % 32 == 0 and d["src0"] == c["dst"] and d["c0"] == 32 and d["cout"] == 2 and c["relu"] == 1)
 
 
-def pack_weights(state_dicts, builder, ops, dtype, q6=False):
+def pack_weights(state_dicts, builder, ops, dtype, q6=False, int8=False):
     """-> (weights tensor [engine dtype], bias tensor fp32, ops with w_off / b_off / wq_off filled)."""
     import torch
+
+    from . import int8 as int8_weights
 
     sds = [{(k[7:] if k.startswith("module.") else k): v for k, v in sd.items()} for sd in state_dicts]
     tdt = {_hip.RCV_F32: torch.float32, _hip.RCV_BF16: torch.bfloat16, _hip.RCV_F16: torch.float16,
@@ -393,6 +408,7 @@ def pack_weights(state_dicts, builder, ops, dtype, q6=False):
         ws, bs, wq, bq = [], [], [], []
         want_q6 = bool(q6) and dtype == _hip.RCV_F16X3 and q6_wanted(spec, op, Q6_DEFAULT if q6 is True else q6)
         want_tailc = dtype == _hip.RCV_F16X3 and tail_composed_wanted(builder, idx)
+        want_int8 = bool(int8) and dtype in (_hip.RCV_BF16, _hip.RCV_F16) and int8_wanted(spec, op, INT8_DEFAULT if int8 is True else int8)
         for sd in sds:
             w, b = fold_conv_bn(sd, spec, op["cout"])
             wmax = float(w.abs().max()) if w.numel() else 0.0
@@ -411,6 +427,10 @@ def pack_weights(state_dicts, builder, ops, dtype, q6=False):
             else:
                 ws.append(w.reshape(-1))
                 bs.append(b)
+                if want_int8:  # codes [cout][taps][channels padded] as 16-bit elements, and the channels' scales
+                    packed = int8_weights.quantize_weight(w[:, 0, 0] if op["ksize"] == 1 else w)
+                    wq.append(packed.codes.reshape(-1).view(tdt))
+                    bq.append(packed.scales)
         wcat = torch.cat(ws).to(tdt)
         bcat = torch.cat(bs + bq).to(torch.float32)  # (second-copy records of all networks BEHIND the first-copy records: strides unchanged)
         op["w_off"], op["b_off"] = woff, boff
@@ -424,9 +444,9 @@ def pack_weights(state_dicts, builder, ops, dtype, q6=False):
         bparts.append(bcat)
         woff += wcat.numel()
         boff += bcat.numel()
-        if wq:  # the second copy of all groups (q6 rows: same strides as the first copy; parity-composed tail: four times the rows)
+        if wq:  # the second copy of all groups (q6 rows: same strides as the first copy; parity-composed tail: four times the rows; int8: its own)
             qcat = torch.cat(wq)
-            assert qcat.numel() % 64 == 0 and (want_tailc or qcat.numel() + pad == wcat.numel())
+            assert qcat.numel() % 64 == 0 and (want_tailc or want_int8 or qcat.numel() + pad == wcat.numel())
             op["wq_off"] = woff
             wparts.append(qcat)
             woff += qcat.numel()
@@ -453,9 +473,11 @@ class FcnEngine:
     q6 (f16x3 only; default off): True or a regex over convolution names -- those stride-1 3x3 convolutions run the cross terms of
     the split product as one block-scaled fp6 matrix instruction (engine option 11, q6_wanted): -18 % on those launches, -3 % on
     the forward, for 2-3x the map error (worst network of the bench 3.4e-5 -> 7.8e-5 of the 1e-4 tolerance: r05 measurement).
+    int8 (bf16 / fp16; default off): True or a regex over convolution names -- those stride-1 convolutions run on 8-bit integers with one
+    scale per pixel and output channel (engine option 16, int8_wanted).
     """
 
-    def __init__(self, state_dicts, H, W, dtype="bf16", device="cuda", reuse_slots=True, arch="dense", q6=False):
+    def __init__(self, state_dicts, H, W, dtype="bf16", device="cuda", reuse_slots=True, arch="dense", q6=False, int8=False):
         import torch
 
         self.lib = _hip.lib()
@@ -467,10 +489,12 @@ class FcnEngine:
         if arch not in ("dense", "res"):
             raise ValueError("arch must be 'dense' (DenseFCNResNet152) or 'res' (ResFCNResNet152)")
         self.arch = arch
+        if int8 and self.dtype not in (_hip.RCV_BF16, _hip.RCV_F16):
+            raise ValueError("int8 convolutions need an engine of 16-bit storage: dtype 'bf16' or 'fp16'")
         builder = build_program(self.H, self.W) if arch == "dense" else build_program_res(self.H, self.W)
         ops, slot_sizes = assign_slots(builder, reuse=reuse_slots)
         self.stages = builder.named if not reuse_slots else {}
-        w, b, ops = pack_weights(state_dicts, builder, ops, self.dtype, q6=q6)
+        w, b, ops = pack_weights(state_dicts, builder, ops, self.dtype, q6=q6, int8=int8)
         self.ops = ops
         self.slot_sizes = slot_sizes
         self.weights = w.to(device)

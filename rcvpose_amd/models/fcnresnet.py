@@ -82,13 +82,18 @@ class DenseFCNResNet152(nn.Module):
         # "fp32": exact-fp32 MFMA kernels (v_mfma_f32_16x16x4_f32)
         # "bf16" / "fp16": 16-bit storage / fp32 accumulate (throughput modes outside the 1e-4 tolerance)
         self.compute_dtype = "f16x3"
+        self.int8 = False
         self._engine = None
         self._engine_key = None
 
-    def set_compute_dtype(self, name):
+    def set_compute_dtype(self, name, int8=False):
+        """int8 ('bf16' / 'fp16' only): the decoder's wide convolutions (True) or those a regex names run on 8-bit integers."""
         if name not in ("f16x3", "fp32", "bf16", "fp16"):
             raise ValueError("compute dtype must be 'f16x3', 'fp32', 'bf16' or 'fp16'")
+        if int8 and name not in ("bf16", "fp16"):
+            raise ValueError("int8 convolutions need compute dtype 'bf16' or 'fp16'")
         self.compute_dtype = name
+        self.int8 = int8
         return self
 
     def _stamp(self):
@@ -98,9 +103,9 @@ class DenseFCNResNet152(nn.Module):
         return v
 
     def engine(self, H, W):
-        key = (H, W, self.compute_dtype, self._stamp())
+        key = (H, W, self.compute_dtype, self.int8, self._stamp())
         if self._engine is None or self._engine_key != key:
-            self._engine = fcn_engine.FcnEngine([self.state_dict()], H, W, dtype=self.compute_dtype, arch=self._arch)
+            self._engine = fcn_engine.FcnEngine([self.state_dict()], H, W, dtype=self.compute_dtype, arch=self._arch, int8=self.int8)
             # the module is the per-call (synchronous) boundary: half-precision storage modes fail loudly on overflow
             self._engine.check_finite = self.compute_dtype != "fp32"
             self._engine_key = key
@@ -148,5 +153,6 @@ class ResFCNResNet152(DenseFCNResNet152):
         self.conv7 = _decoder_stage(128, 64)
         self.conv8 = nn.Conv2d(64, output_channels, kernel_size=1, stride=1)
         self.compute_dtype = "f16x3"
+        self.int8 = False
         self._engine = None
         self._engine_key = None

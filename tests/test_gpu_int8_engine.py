@@ -1,0 +1,139 @@
+"""FcnEngine(int8=...): chosen convolutions of the FCN on 8-bit integers (engine option 16 of the 16-bit engines, rcv_op::wq_off)."""
+import ctypes
+import json
+import os
+
+import pytest
+import torch
+
+import fcn_weights
+from rcvpose_amd import _hip, fcn_engine, int8
+from rcvpose_amd.fcn_engine import FcnEngine
+
+pytestmark = pytest.mark.gpu
+
+TORCH = {"bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+@pytest.fixture(scope="module")
+def sds(golden_dir):
+    shapes = json.load(open(os.path.join(golden_dir, "fcn_state_dict_keys.json")))
+    return [{k: torch.from_numpy(v) for k, v in fcn_weights.make_state_dict_numpy(shapes, seed=s).items()} for s in range(2)]
+
+
+@pytest.fixture(scope="module")
+def x():
+    return torch.randn(3, 3, 64, 96, generator=torch.Generator().manual_seed(1)).cuda()
+
+
+# one name per kind of op: long 3x3, 3x3 over two sources, a 3x3 in the middle of a bottleneck, 1x1 with and without a residual, the
+# 3x3 between the last upsampling and the head
+NAMES = ["conv6", "conv_up4.0", "conv_up1.0", "block2.3.conv2", "block3.7.conv1", "block4.1.conv3", "block4up.conv3", "conv7.0"]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_every_int8_op_equals_the_public_operators(sds, x, dtype):
+    """The engine's op, from the stored activations: quantize_tokens + matmul / conv3x3 with the folded weights.  Groups may divide a sum
+    differently (float32 additions in another order), so a value may round to the neighbouring 16-bit number."""
+    eng = FcnEngine(sds, 64, 96, dtype=dtype, reuse_slots=False, int8="|".join(n.replace(".", r"\.") for n in NAMES))
+    eng.forward(x)
+    builder = fcn_engine.build_program(64, 96)
+    seen = []
+    for op, spec in zip(eng.ops, builder.wspecs):
+        if not op["wq_off"]:
+            continue
+        seen.append(spec["conv"])
+        for g in range(2):
+            def get(slot, h, w, c):
+                return None if slot < 0 else eng.debug_slot(3, g, slot, (h, w, c)).to(TORCH[dtype])
+            src0, src1 = get(op["src0"], op["hin"], op["win"], op["c0"]), get(op["src1"], op["hin"], op["win"], op["c1"])
+            res, got = get(op["res"], op["hout"], op["wout"], op["cout"]), get(op["dst"], op["hout"], op["wout"], op["cout"])
+            w, b = fcn_engine.fold_conv_bn(sds[g], spec, op["cout"])
+            weight = int8.quantize_weight(w[:, 0, 0] if op["ksize"] == 1 else w).to("cuda")
+            call = int8.matmul if op["ksize"] == 1 else int8.conv3x3
+            codes, scales = int8.quantize_tokens(src0, src1)
+            want = call(codes, scales, weight, bias=b.float().cuda(), residual=res, relu=bool(op["relu"]), dtype=TORCH[dtype]).double()
+            # Both are within 31 roundings of float32 (nine taps, up to sixteen partial sums, scale, bias, residual) of the same real number, a
+            # rounding being at most 2^-24 of the sum of the magnitudes that are added; so they differ by twice that, and each is then
+            # rounded by at most half a step of its type: eps / 2 of its value, or half of the smallest subnormal.
+            size = call(codes.abs(), scales, int8.pack_codes(weight.codes[:, :, :weight.channels].abs().reshape(w.shape if op["ksize"] == 3 else w[:, 0, 0].shape),
+                                                            weight.scales), bias=b.float().abs().cuda(),
+                        residual=None if res is None else res.float().abs(), dtype=torch.float32).double()
+            eps = torch.finfo(TORCH[dtype]).eps
+            diff = (got.double() - want).abs()
+            assert bool((diff <= 62 * 2.0 ** -24 * size * (1 + eps) + eps * want.abs() * (1 + eps) + 2.0 ** -24).all()), (spec["conv"], g, float(diff.max()))
+            assert float((diff > 0).double().mean()) < 1e-2
+            assert float(want.abs().max()) > 0
+    assert sorted(seen) == sorted(NAMES)
+
+
+def test_option_16_switches_back(sds, x):
+    plain = FcnEngine(sds, 64, 96, dtype="bf16").forward(x)
+    eng = FcnEngine(sds, 64, 96, dtype="bf16", int8=True)
+    seg, rad = eng.forward(x)
+    assert bool(torch.isfinite(rad).all()) and not torch.equal(rad, plain[1])
+    assert float((rad - plain[1]).abs().max()) < 0.5 * float(plain[1].abs().max())
+    again = eng.forward(x)
+    assert torch.equal(again[0], seg) and torch.equal(again[1], rad)
+    eng.set_option(16, 0)
+    off = eng.forward(x)
+    assert torch.equal(off[0], plain[0]) and torch.equal(off[1], plain[1])
+
+
+def test_captured_forward_equals_eager(sds, x):
+    eng = FcnEngine(sds, 64, 96, dtype="fp16", int8=True)
+    seg, rad = [t.clone() for t in eng.forward(x)]
+    graph, gs, gr = eng.capture(x)
+    for _ in range(3):
+        gs.zero_(), gr.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(gs, seg) and torch.equal(gr, rad)
+        assert torch.equal(eng.forward(x)[1], rad)
+    assert eng.range_status() == 0
+
+
+def test_fp16_overflow_of_an_int8_op_is_reported(sds, x):
+    sd = dict(sds[0])
+    sd["conv6.bias"] = sd["conv6.bias"] + 1e9  # (bn6 scales it back down, but not below 65504)
+    eng = FcnEngine([sd], 64, 96, dtype="fp16", int8=r"conv6")
+    eng.forward(x)
+    assert eng.range_status(clear=True) & 2
+    with pytest.raises(_hip.HalfRangeError):
+        eng.forward(x)
+        eng.range_status(raise_on_flag=True)
+
+
+def test_model_and_refusals(sds, x):
+    from rcvpose_amd.models.fcnresnet import DenseFCNResNet152
+
+    m = DenseFCNResNet152(3, 2).eval()
+    m.load_state_dict(sds[0])
+    m.set_compute_dtype("bf16", int8=True)
+    seg, rad = m(x)
+    ref = FcnEngine(sds[:1], 64, 96, dtype="bf16", int8=True).forward(x)
+    assert torch.equal(seg, ref[0][0]) and torch.equal(rad, ref[1][0])
+    with pytest.raises(ValueError):
+        FcnEngine(sds[:1], 64, 96, dtype="f16x3", int8=True)
+
+    lib = _hip.lib()
+    w = torch.zeros(1 << 16, dtype=torch.bfloat16, device="cuda")
+    bias = torch.zeros(1024, device="cuda")
+    base = dict(kind=_hip.OP_CONV, src0=0, src1=-1, res=-1, dst=1, c0=64, cout=64, hin=8, win=8, hout=8, wout=8, ksize=3, stride=1, pad=1, w_off=0,
+                b_off=0, wq_off=40960)
+    for change, status in ((dict(), _hip.RCV_OK), (dict(stride=2, hout=4, wout=4), _hip.RCV_E_UNSUPPORTED), (dict(ksize=5, pad=2), _hip.RCV_E_UNSUPPORTED),
+                           (dict(pad=0, hout=6, wout=6), _hip.RCV_E_UNSUPPORTED), (dict(wq_off=40961), _hip.RCV_E_INVALID),
+                           (dict(src0=_hip.SLOT_INPUT), _hip.RCV_E_INVALID)):
+        op = _hip.Op(**{**base, **change})
+        handle = ctypes.c_void_p()
+        slots = (ctypes.c_int64 * 2)(64 * 64, 64 * 64)
+        rc = lib.rcv_fcn_create(ctypes.byref(op), 1, 2, slots, 1, _hip.RCV_BF16, w.data_ptr(), bias.data_ptr(), ctypes.byref(handle))
+        assert rc == status, change
+        if rc == _hip.RCV_OK:
+            plain = _hip.Op(**{**base, "wq_off": 0})
+            h2 = ctypes.c_void_p()
+            _hip.check(lib.rcv_fcn_create(ctypes.byref(plain), 1, 2, slots, 1, _hip.RCV_BF16, w.data_ptr(), bias.data_ptr(), ctypes.byref(h2)))
+            # the scratch of the codes is part of the workspace: 4 images of 64 pixels x 64 codes and a scale each
+            assert lib.rcv_fcn_workspace_bytes(handle, 4) >= lib.rcv_fcn_workspace_bytes(h2, 4) + 4 * 64 * (64 + 4)
+            lib.rcv_fcn_destroy(h2)
+            lib.rcv_fcn_destroy(handle)

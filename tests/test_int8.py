@@ -120,3 +120,57 @@ def test_no_cpu_fallback():
         int8.quantize_tokens(torch.ones(2, 4))
     with pytest.raises(_hip.HipLibraryError):
         int8.matmul(torch.ones(2, 4, dtype=torch.int8), torch.ones(2), int8.quantize_weight(torch.ones(3, 4)))
+
+
+def test_engine_weights_with_an_int8_copy():
+    """pack_weights(int8=...): codes and scales of the matching convolutions behind the 16-bit copy, every other op as without."""
+    import json
+    import os
+
+    import fcn_weights
+    from rcvpose_amd import fcn_engine
+
+    golden = os.path.join(os.path.dirname(os.path.abspath(__file__)), "golden")
+    shapes = json.load(open(os.path.join(golden, "fcn_state_dict_keys.json")))
+    sds = [{k: torch.from_numpy(v) for k, v in fcn_weights.make_state_dict_numpy(shapes, seed=s).items()} for s in range(2)]
+    b = fcn_engine.build_program(64, 96)
+    names = ["conv_up3.0", "block4.1.conv3"]
+    w0, b0, ops0 = fcn_engine.pack_weights(sds, b, fcn_engine.assign_slots(b)[0], _hip.RCV_BF16)
+    w1, b1, ops1 = fcn_engine.pack_weights(sds, b, fcn_engine.assign_slots(b)[0], _hip.RCV_BF16, int8="|".join(n.replace(".", r"\.") for n in names))
+    seen = []
+    for o0, o1, spec in zip(ops0, ops1, b.wspecs):
+        assert o0["wq_off"] == 0
+        if spec is None:
+            continue
+        k = o1["c0"] + (o1["c1"] if o1["src1"] >= 0 else 0)
+        n_w = 2 * o1["cout"] * o1["ksize"] ** 2 * k
+        assert torch.equal(w0[o0["w_off"]:o0["w_off"] + n_w].view(torch.int16), w1[o1["w_off"]:o1["w_off"] + n_w].view(torch.int16))
+        assert torch.equal(b0[o0["b_off"]:o0["b_off"] + 2 * o1["cout"]], b1[o1["b_off"]:o1["b_off"] + 2 * o1["cout"]])
+        if spec["conv"] not in names:
+            assert o1["wq_off"] == 0
+            continue
+        seen.append(spec["conv"])
+        taps, kp = o1["ksize"] ** 2, -(-k // 128) * 128
+        assert o1["wq_off"] % 8 == 0
+        codes = w1[o1["wq_off"]:o1["wq_off"] + o1["cout"] * taps * kp].view(torch.int8).view(2, o1["cout"], taps, kp)
+        scales = b1[o1["b_off"] + 2 * o1["cout"]:o1["b_off"] + 4 * o1["cout"]].view(2, o1["cout"])
+        for g in range(2):
+            w, _ = fcn_engine.fold_conv_bn(sds[g], spec, o1["cout"])
+            q = int8.quantize_weight(w[:, 0, 0] if taps == 1 else w)
+            assert torch.equal(codes[g], q.codes) and torch.equal(scales[g], q.scales)
+    assert sorted(seen) == sorted(names)
+    # the split-precision engine's second copies stay what they are
+    assert fcn_engine.pack_weights(sds[:1], b, fcn_engine.assign_slots(b)[0], _hip.RCV_F16X3, int8=True)[0].numel() == \
+        fcn_engine.pack_weights(sds[:1], b, fcn_engine.assign_slots(b)[0], _hip.RCV_F16X3)[0].numel()
+
+
+def test_model_takes_int8_with_16_bit_types_only():
+    from rcvpose_amd.models.fcnresnet import DenseFCNResNet152
+
+    m = DenseFCNResNet152(3, 2)
+    assert m.set_compute_dtype("bf16", int8=True).int8 is True
+    assert m.set_compute_dtype("fp16").int8 is False
+    for name in ("f16x3", "fp32"):
+        with pytest.raises(ValueError):
+            m.set_compute_dtype(name, int8=True)
+    assert m.compute_dtype == "fp16"
