@@ -104,8 +104,8 @@ def _elsewhere(t):
     raise ValueError("all tensors of a call must be on one device")
 
 
-def _launch(index, name, fn, *args):
-    """fn(*args, stream) with device `index` current, on that device's current stream."""
+def _call(index, name, fn, *args):
+    """fn(*args, stream) on device `index`'s current stream."""
     if _current_device() == index:
         rc = fn(*args, _raw_stream(index))
     else:
@@ -146,12 +146,12 @@ def quantize_tokens(x, x1=None):
     lead = shape[:-1]
     codes, scales = x.new_empty(lead + (pitch,), dtype=torch.int8), x.new_empty(lead, dtype=torch.float32)
     if rows:
-        _launch(index, "rcv_i8_quantize_tokens", L.rcv_i8_quantize_tokens, x.data_ptr(), pitch0, c0, x1_ptr, pitch1, c1, dtype, rows,
+        _call(index, "rcv_i8_quantize_tokens", L.rcv_i8_quantize_tokens, x.data_ptr(), pitch0, c0, x1_ptr, pitch1, c1, dtype, rows,
                 codes.data_ptr(), pitch, scales.data_ptr())
     return codes if pitch == c else codes[..., :c], scales
 
 
-def _product(name, codes, scales, weight, bias, residual, relu, dtype, height, width):
+def _product(codes, scales, weight, bias, residual, relu, dtype, height, width):
     L = _hip.load_library()
     k, n, shape = weight.channels, weight.out_channels, codes.shape
     lead = shape[:-1]
@@ -165,19 +165,23 @@ def _product(name, codes, scales, weight, bias, residual, relu, dtype, height, w
     index = codes.get_device()
     if index < 0:
         _elsewhere(codes)
-    for t in (scales, weight.codes, weight.scales, bias, residual):
-        if t is not None and t.get_device() != index:
-            _elsewhere(t)
+    wcodes, wscales = weight.codes, weight.scales
+    if scales.get_device() != index or wcodes.get_device() != index or wscales.get_device() != index:
+        _elsewhere(next(t for t in (scales, wcodes, wscales) if t.get_device() != index))
     out = codes.new_empty(lead + (n,), dtype=dtype)
     bias_ptr = res_ptr = res_pitch = 0
     if bias is not None:
-        if bias.dtype != torch.float32 or bias.shape != (n,):
+        if bias.dtype != torch.float32 or bias.dim() != 1 or bias.shape[0] != n:
             raise ValueError("bias must be float32 [%d]" % n)
+        if bias.get_device() != index:
+            _elsewhere(bias)
         bias = bias.contiguous()
         bias_ptr = bias.data_ptr()
     if residual is not None:
         if residual.dtype != dtype or residual.shape != out.shape:
             raise ValueError("residual must have the output's type and shape")
+        if residual.get_device() != index:
+            _elsewhere(residual)
         residual, _, res_pitch = _rows(residual)
         res_ptr = residual.data_ptr()
     codes, rows, pitch = _rows(codes)
@@ -190,11 +194,15 @@ def _product(name, codes, scales, weight, bias, residual, relu, dtype, height, w
         raise ValueError("token rows must start 16 bytes aligned and be readable up to a multiple of 16 channels: "
                          "take the codes as quantize_tokens lays them out")
     scales = scales.contiguous()
-    args = _pack_args(_ARGS_BYTES, out_type, ptr, scales.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(), bias_ptr, res_ptr,
+    args = _pack_args(_ARGS_BYTES, out_type, ptr, scales.data_ptr(), wcodes.data_ptr(), wscales.data_ptr(), bias_ptr, res_ptr,
                       out.data_ptr(), rows, pitch, res_pitch, n, k, n, height, width, 1 if relu else 0, 0)
-    nbytes = getattr(L, name + "_workspace_bytes")(rows, k, n)
-    ws = codes.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    _launch(index, name, getattr(L, name), args, None if ws is None else ws.data_ptr(), nbytes)
+    call, workspace_bytes = (L.rcv_i8_conv3x3, L.rcv_i8_conv3x3_workspace_bytes) if height else (L.rcv_i8_matmul, L.rcv_i8_matmul_workspace_bytes)
+    nbytes = workspace_bytes(rows, k, n)
+    if nbytes:
+        ws = codes.new_empty(nbytes, dtype=torch.uint8)
+        _call(index, "int8 product", call, args, ws.data_ptr(), nbytes)
+    else:
+        _call(index, "int8 product", call, args, None, 0)
     return out
 
 
@@ -205,7 +213,7 @@ def matmul(codes, scales, weight, bias=None, residual=None, relu=False, dtype=to
     residual [..., N] of `dtype`.  The integer sums are exact; the result is rounded once, to `dtype`.  relu keeps a NaN."""
     if weight.taps != 1:
         raise ValueError("matmul takes a weight packed from [N, K]; a 3x3 weight belongs to conv3x3")
-    return _product("rcv_i8_matmul", codes, scales, weight, bias, residual, relu, dtype, 0, 0)
+    return _product(codes, scales, weight, bias, residual, relu, dtype, 0, 0)
 
 
 def conv3x3(codes, scales, weight, bias=None, residual=None, relu=False, dtype=torch.bfloat16):
@@ -216,4 +224,4 @@ def conv3x3(codes, scales, weight, bias=None, residual=None, relu=False, dtype=t
         raise ValueError("conv3x3 takes a weight packed from [N, 3, 3, C]")
     if codes.dim() != 4:
         raise ValueError("codes must be int8 [B, H, W, C]")
-    return _product("rcv_i8_conv3x3", codes, scales, weight, bias, residual, relu, dtype, codes.shape[1], codes.shape[2])
+    return _product(codes, scales, weight, bias, residual, relu, dtype, codes.shape[1], codes.shape[2])
