@@ -395,18 +395,24 @@ template <typename T, int TAPS> __global__ __launch_bounds__(256) void k_i8_fini
 // operands through LDS
 // ---------------------------------------------------------------------------------------------
 
-// One piece of an operand tile: 64 lanes x 16 bytes from `rsrc` + soff + voff to LDS bytes [lds + LDS_OFF, + 1024).  Lanes whose offset (soff
-// included) is not below the descriptor's size deliver zeros.  (Inline: the compiler would wait for every piece before the next LDS
-// read of any stage.  The instruction has no register result; the kernel counts the pieces itself.)
-template <int LDS_OFF> __device__ __forceinline__ void dma16(i32x4 rsrc, int soff, unsigned lds, int voff)
+// One piece of an operand tile: 64 lanes x 16 bytes from `at` + soff + voff to LDS bytes [lds + LDS_OFF, + 1024).  Lanes whose offset (soff
+// included) is not below `bytes` deliver zeros.
+struct View {
+    long long at;
+    int bytes;
+};
+template <int LDS_OFF> __device__ __forceinline__ void dma16(const View &v, int soff, unsigned lds, int voff)
 {
-    asm volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc), "s"(soff),
-                 "n"(LDS_OFF)
-                 : "m0", "scc");
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void *)v.at, 0, v.bytes, 0x00020000),
+                                             (__attribute__((address_space(3))) void *)(uintptr_t)(lds + LDS_OFF), 16, voff, soff, 0, 0);
 }
-template <int N> __device__ __forceinline__ void wait_pieces()  // all but the newest N pieces of this wave have landed, and its LDS reads are done
+// All but the newest N pieces of every wave have landed, and all LDS reads before are done.  (The compiler does not wait for the pieces: it
+// does not connect them with the reads.  It moves no access to memory past either statement.)
+template <int N> __device__ __forceinline__ void step_barrier()
 {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
 template <int I, int N, typename F> __device__ __forceinline__ void for_each(F &&f)  // f(I) ... f(N - 1), each a compile-time constant
@@ -546,7 +552,7 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_i8_tile(const I8Product p, in
     const unsigned a_last = a_lds + (S::NA - 1) * S::A_BYTES, b_last = b_lds + (S::NB - 1) * S::B_BYTES;
     // The descriptors of a tap, in few scalar instructions (every wave runs them, all matrix units wait): the tokens move by `shift` rows, and
     // the view ends with the tile's or the tensor's last row, whichever comes first.
-    i32x4 ra, rb;
+    View ra, rb;
     const long long next_col = pitch, next_row = (long long)(W - 2) * pitch;
     const int below = (int)min(p.rows - m0, 1LL << 30), last_row = (int)pitch - ((p.K + 15) & ~15);
     long long a_at = (long long)(codes + (m0 + (TAPS == 9 ? (long long)(tap0 / 3 - 1) * W + (tap0 % 3 - 1) : 0)) * pitch);
@@ -555,9 +561,9 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_i8_tile(const I8Product p, in
     int b_bytes = min(p.Cout - n0, BN) * wrow - tap0 * p.kp;
     auto a_view = [&]() {
         const int rows = min(below - shift, BM);
-        ra = i32x4{(int)a_at, (int)(a_at >> 32) & 0xffff, rows > 0 ? rows * (int)pitch - last_row : 0, 0x00020000};
+        ra = View{a_at, rows > 0 ? rows * (int)pitch - last_row : 0};
     };
-    auto b_view = [&]() { rb = i32x4{(int)b_at, (int)(b_at >> 32) & 0xffff, b_bytes, 0x00020000}; };
+    auto b_view = [&]() { rb = View{b_at, b_bytes}; };
     auto a_tap = [&]() {
         const bool wrap = ++a_col == 3;
         a_col = wrap ? 0 : a_col;
@@ -591,7 +597,6 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_i8_tile(const I8Product p, in
 
     a_view();
     b_view();
-    asm volatile("s_nop 4");  // (scalars that came through vector registers, before the first piece reads them)
     for (int s = 0; s < S::NA - 1; s++) {  // tokens of steps 0 .. NA - 2 and weights of steps 0 .. NB - 1 in the order of the loop
         for_each<0, PA>(a_piece);
         a_end();
@@ -646,6 +651,12 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_i8_tile(const I8Product p, in
 #pragma unroll
             for (int q = 0; q < NF; q++) if (q * RSEG / NF == s) read(1 - f, half, q);
             for_each<s * n / SEG, (s + 1) * n / SEG>(piece);
+            // (reads, half of the products, a piece, the others: with its addresses computed under the first two products a piece costs less
+            // than in the compiler's order, 518 against 526 us at 60 x 80 x 53 and 1024 -> 256 channels)
+            __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
 #pragma unroll
             for (int e = s * 4; e < s * 4 + 4; e++) {
                 const int i = e / TT, j = e % TT;
@@ -659,16 +670,14 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_i8_tile(const I8Product p, in
     constexpr std::integral_constant<int, PA> pa{};
     constexpr std::integral_constant<int, PB> pb{};
 
-    wait_pieces<S::LATE + PB>();
-    __builtin_amdgcn_s_barrier();
+    step_barrier<S::LATE + PB>();
 #pragma unroll
     for (int q = 0; q < NF; q++) read(0, 0, q);
     for (int tap = tap0; tap < tap1; tap++) {
         for (int k = klo; k < khi; k += KB) {
             multiply(c0, 1, pa, a_piece);
             a_end();
-            wait_pieces<S::LATE>();  // the next step is here; nobody reads the current one any more
-            __builtin_amdgcn_s_barrier();
+            step_barrier<S::LATE>();  // the next step is here; nobody reads the current one any more
             a_stage = a_stage == (S::NA - 1) * S::A_BYTES ? 0 : a_stage + S::A_BYTES;
             b_stage = b_stage == (S::NB - 1) * S::B_BYTES ? 0 : b_stage + S::B_BYTES;
             multiply(c1, 0, pb, b_piece);
@@ -803,9 +812,10 @@ Plan plan_product(long long rows, int K, int Cout, int taps, int groups)
 {
     Plan pl{Plan::SQUARE, 1, 0};
     const int steps = taps * ((K + 127) / 128);
-    if (rows <= 64) {
+    const long long small = tile_count(rows, Cout, groups, 64, 16);
+    if (rows <= 64 || (small <= (taps == 9 ? 480 : 320) && small * 80 * taps * i8_kp(K) <= 60000000)) {
         pl.kind = Plan::DIRECT;
-        const long long wgs = tile_count(rows, Cout, groups, 64, 16);
+        const long long wgs = small;
         while (wgs * pl.splits * 2 <= 256 && steps >= pl.splits * 2 * 16) pl.splits *= 2;  // (at least four 64-channel steps a wave)
     } else {
         // rounds of the chip's 256 CUs times the relative time of a tile
