@@ -441,7 +441,8 @@ int rcv_fcn_get_op_times(rcv_fcn *h, double *ms_out, int n_ops);
  * RCV_BF16 / RCV_F16), rows pitch0 / pitch1 elements apart (x1_dev NULL and c1 = 0: one).  scale = f32(max |x| / 127), code =
  * round-half-even of the exact quotient x / scale, so codes are -127 .. 127.  A row whose scale falls below 2^-126, the all-zero row
  * among them, gets scale 0 and codes 0; a row with a NaN or an infinity gets scale NaN and codes 0, which makes every
- * product with it NaN.  Bytes between a row's last code and its pitch are left alone.
+ * product with it NaN.  Bytes between a row's last code and its pitch are left alone.  c0 + c1 <= 131071, rows < 2^31 and pitches up
+ * to 2^24, else RCV_E_TOO_LARGE.
  */
 int rcv_i8_quantize_tokens(const void *x0_dev, long long pitch0, int c0, const void *x1_dev, long long pitch1, int c1, int dtype,
                            long long rows, int8_t *codes_dev, long long codes_pitch, float *scales_dev, void *stream);
@@ -457,7 +458,8 @@ int rcv_i8_quantize_tokens(const void *x0_dev, long long pitch0, int c0, const v
  *   weights     [out_channels][taps][channels rounded up to a multiple of 128], 16-byte aligned, zeros behind `channels`
  *   bias        [out_channels] or NULL; residual [rows, residual_pitch] of out_dtype or NULL (may be `out` itself)
  *   ws          device scratch of rcv_i8_*_workspace_bytes (0 where every call of that size runs without)
- * channels <= 131071 (no sum can overflow), else RCV_E_TOO_LARGE.  rows = 0 does nothing.
+ * rows = 0 does nothing.  RCV_E_TOO_LARGE: channels > 131071 (a sum could overflow), out_channels > 2^20, width > 2^16, more rows than a
+ * launch has threads for (2^30 with up to 128 output channels), codes_pitch > 2^22 or a pitch of more than 2^24 elements.
  */
 typedef struct rcv_i8_args {
     uint32_t struct_bytes;     /* sizeof(rcv_i8_args) of the caller's header: RCV_E_INVALID when it is another's */

@@ -652,7 +652,7 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_i8_tile(const I8Product p, in
             for (int q = 0; q < NF; q++) if (q * RSEG / NF == s) read(1 - f, half, q);
             for_each<s * n / SEG, (s + 1) * n / SEG>(piece);
             // (reads, half of the products, a piece, the others: with its addresses computed under the first two products a piece costs less
-            // than in the compiler's order, 518 against 526 us at 60 x 80 x 53 and 1024 -> 256 channels)
+            // than in the compiler's order: 518 against 526 us for the window over 53 images of 30 x 40, 2048 -> 512 channels)
             __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
             __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
             __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
@@ -768,13 +768,20 @@ int launch_quantize(const void *x0_, long long pitch0, int c0, const void *x1_, 
     const T *x0 = (const T *)x0_, *x1 = (const T *)x1_;
     const int C = c0 + c1;
     const bool aligned = (uintptr_t)codes % 16 == 0 && codes_pitch % 16 == 0;
+    // a launch holds fewer than 2^32 threads: `per` tokens at most
+    auto in_parts = [&](long long per, auto &&launch) -> int {
+        for (long long r = 0; r < rows; r += per) {
+            launch(x0 + r * pitch0, x1 ? x1 + r * pitch1 : x1, std::min(per, rows - r), codes + r * codes_pitch, scales + r);
+            RCV_LAUNCH_CHECK();
+        }
+        return RCV_OK;
+    };
 #define RCV_I8_Q(L, NV)                                                                                                           \
-    if (C <= L * NV * 16) {                                                                                                       \
-        hipLaunchKernelGGL((k_i8_quantize<T, L, NV>), dim3((unsigned)((rows + 256 / L - 1) / (256 / L))), dim3(256), 0, st, x0, pitch0, c0, \
-                           x1, pitch1, c1, rows, codes, codes_pitch, scales, aligned);                                            \
-        RCV_LAUNCH_CHECK();                                                                                                       \
-        return RCV_OK;                                                                                                            \
-    }
+    if (C <= L * NV * 16)                                                                                                         \
+        return in_parts((1LL << 31) / L, [&](const T *a, const T *b, long long n, int8_t *q, float *s) {                          \
+            hipLaunchKernelGGL((k_i8_quantize<T, L, NV>), dim3((unsigned)((n + 256 / L - 1) / (256 / L))), dim3(256), 0, st, a, pitch0, c0, b, \
+                               pitch1, c1, n, q, codes_pitch, s, aligned);                                                        \
+        });
     RCV_I8_Q(4, 1)
     RCV_I8_Q(16, 1)
     RCV_I8_Q(32, 1)
@@ -782,10 +789,9 @@ int launch_quantize(const void *x0_, long long pitch0, int c0, const void *x1_, 
     RCV_I8_Q(64, 2)
     RCV_I8_Q(64, 4)
 #undef RCV_I8_Q
-    hipLaunchKernelGGL((k_i8_quantize_long<T>), dim3((unsigned)rows), dim3(1024), 0, st, x0, pitch0, c0, x1, pitch1, c1, codes, codes_pitch,
-                       scales, aligned);
-    RCV_LAUNCH_CHECK();
-    return RCV_OK;
+    return in_parts((1LL << 31) / 1024, [&](const T *a, const T *b, long long n, int8_t *q, float *s) {
+        hipLaunchKernelGGL((k_i8_quantize_long<T>), dim3((unsigned)n), dim3(1024), 0, st, a, pitch0, c0, b, pitch1, c1, q, codes_pitch, s, aligned);
+    });
 }
 
 // Lets `kernel` use more than the default 64 KB of LDS on the current device, once (ready: one bit per device).
@@ -849,11 +855,11 @@ template <typename T, int TAPS> int launch_finish(const I8Product &p, const Plan
 
 template <typename T, typename S> int launch_tile(const I8Product &p, const Plan &pl, void *ws, hipStream_t st)
 {
+    const long long tm = (p.rows + S::BM - 1) / S::BM, tn = (p.Cout + S::BN - 1) / S::BN;
+    if (tm * tn * 64 * S::NW > 0xffffffffLL) return RCV_E_TOO_LARGE;  // (threads of a launch)
     static std::atomic<unsigned long long> ready{0};
     const int rc = allow_lds((const void *)k_i8_tile<T, S>, S::LDS, ready);
     if (rc != RCV_OK) return rc;
-    const long long tm = (p.rows + S::BM - 1) / S::BM, tn = (p.Cout + S::BN - 1) / S::BN;
-    if (tm * tn > 0x7fffffffLL) return RCV_E_TOO_LARGE;
     f32x4 *partial = S::SPLIT ? (f32x4 *)ws : nullptr;
     hipLaunchKernelGGL((k_i8_tile<T, S>), dim3((unsigned)(tm * tn), pl.splits, p.groups), dim3(64 * S::NW), S::LDS, st, p, (int)tm, (int)tn, partial);
     RCV_LAUNCH_CHECK();
@@ -869,7 +875,6 @@ template <typename T, int TAPS, int TT, int CT, int D> int launch_direct(const I
         if (rc != RCV_OK) return rc;
     }
     const long long tm = (p.rows + TT * 16 - 1) / (TT * 16), tn = (p.Cout + CT * 16 - 1) / (CT * 16);
-    if (tm * tn > 0x7fffffffLL) return RCV_E_TOO_LARGE;
     f32x4 *partial = pl.splits > 1 ? (f32x4 *)ws : nullptr;
     hipLaunchKernelGGL((k_i8_direct<T, TAPS, TT, CT, NW, D>), dim3((unsigned)(tm * tn), pl.splits, p.groups), dim3(64 * NW), LDS, st, p, (int)tn,
                        partial);

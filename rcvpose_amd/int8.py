@@ -6,7 +6,7 @@
     y = conv3x3(codes, scales, weight, bias)             # codes [B, H, W, C] -> [B, H, W, N], zero padding, stride 1
 
 A token is one row of a channels-last tensor; its value is codes * scale.  FcnEngine(int8=...) runs chosen convolutions of the FCN on
-these kernels.  Inference only; there is no CPU fallback.  Results do not depend on the run: integer sums are exact and float sums
+these kernels.  Inference only: no gradient flows through; there is no CPU fallback.  Results do not depend on the run: integer sums are exact and float sums
 have a fixed order.  The reference has no counterpart (its forward is fp32, models/fcnresnet.py:121-191).
 """
 import ctypes
@@ -29,6 +29,11 @@ class Int8Weight:
     taps is 1 (matmul) or 9 (conv3x3)."""
 
     def __init__(self, codes, scales, channels):
+        if (codes.dtype != torch.int8 or codes.dim() != 3 or codes.shape[0] == 0 or codes.shape[1] not in (1, 9) or not codes.is_contiguous() or
+                not 1 <= channels <= MAX_CHANNELS or codes.shape[2] != (channels + KP - 1) // KP * KP):
+            raise ValueError("packed weight codes must be contiguous int8 [N, 1 or 9, channels padded to a multiple of %d]: see pack_codes" % KP)
+        if scales.dtype != torch.float32 or tuple(scales.shape) != (codes.shape[0],) or not scales.is_contiguous() or scales.device != codes.device:
+            raise ValueError("weight scales must be contiguous float32 [N] on the codes' device")
         self.codes, self.scales, self.channels = codes, scales, channels
         self.out_channels, self.taps = int(codes.shape[0]), int(codes.shape[1])
 

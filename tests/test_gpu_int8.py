@@ -178,7 +178,9 @@ MATMUL = [(1, 1, 1), (1, 16, 5), (1, 4096, 300), (2, 131, 17), (3, 100, 33), (16
           (777, 1500, 333),
           # enough output tiles for the large-product kernel: many rows of few channels, few rows of many
           (33000, 70, 40), (33023, 200, 9), (300, 150, 16500),
-          (12300, 1030, 1025)]
+          (12300, 1030, 1025),
+          # a long sum over few tiles, divided over workgroups
+          (200, 8200, 900), (70, 20000, 1300)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
@@ -200,7 +202,9 @@ def test_matmul(m, k, n, dtype):
 CONV = [(1, 1, 1, 16, 1), (1, 1, 9, 64, 32), (2, 9, 1, 48, 24), (2, 5, 7, 33, 19), (1, 15, 20, 256, 96), (3, 37, 53, 96, 80), (1, 2, 2, 1, 1),
         (5, 8, 8, 128, 130), (2, 15, 20, 640, 64), (1, 61, 70, 64, 200),
         # enough output tiles for the large-product kernel
-        (9, 61, 70, 33, 24), (7, 47, 101, 130, 120), (7, 47, 101, 40, 136), (33001, 1, 1, 20, 8), (1, 33000, 2, 16, 4)]
+        (9, 61, 70, 33, 24), (7, 47, 101, 130, 120), (7, 47, 101, 40, 136), (33001, 1, 1, 20, 8), (1, 33000, 2, 16, 4),
+        # a long sum over few tiles, divided by taps
+        (1, 13, 21, 1100, 300), (3, 40, 41, 700, 260)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
@@ -245,25 +249,109 @@ def test_codes_inside_a_wider_matrix():
     check_product(got, v, mag, torch.float32, 1)
 
 
-@pytest.mark.parametrize("rows, n, pitch", [(5, 7, 12), (70, 64, 72), (300, 130, 131), (520, 128, 160)])
+@pytest.mark.parametrize("rows, n, pitch", [(5, 7, 12), (70, 64, 72), (300, 130, 131), (520, 128, 160), (2500, 260, 261), (20000, 1100, 1101)])
 def test_output_rows_at_a_pitch(rows, n, pitch):
     """The columns between two rows and the rows behind the last stay as they were, the residual may be the output itself."""
     rng = np.random.default_rng(rows)
     L = _hip.lib()
-    a, sa, w, sw, bias, _ = make(rng, rows, 96, n, 1, torch.bfloat16, False)
+    k = 1056 if n > 1000 else 96  # (the last case is one of the large-product kernel's widest tiles)
+    a, sa, w, sw, bias, _ = make(rng, rows, k, n, 1, torch.bfloat16, False)
     weight = int8.pack_codes(w, sw)
     buf = torch.randn(rows + 2, pitch, device="cuda").bfloat16()
     before = f64(buf)
     args = _hip.I8Args(ctypes.sizeof(_hip.I8Args), _hip.RCV_BF16, a.data_ptr(), sa.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(),
-                       bias.data_ptr(), buf.data_ptr(), buf.data_ptr(), rows, a.stride(0), pitch, pitch, 96, n, 0, 0, 1, 0)
-    need = L.rcv_i8_matmul_workspace_bytes(rows, 96, n)
+                       bias.data_ptr(), buf.data_ptr(), buf.data_ptr(), rows, a.stride(0), pitch, pitch, k, n, 0, 0, 1, 0)
+    need = L.rcv_i8_matmul_workspace_bytes(rows, k, n)
     ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
     _hip.check(L.rcv_i8_matmul(ctypes.byref(args), ws.data_ptr(), need, _hip.current_stream()))
     after = f64(buf)
-    v, mag = ref_product(a.cpu().numpy(), sa.cpu().numpy(), w.cpu().numpy().reshape(n, 1, 96), sw.cpu().numpy(), f64(bias), before[:rows, :n], True)
+    v, mag = ref_product(a.cpu().numpy(), sa.cpu().numpy(), w.cpu().numpy().reshape(n, 1, k), sw.cpu().numpy(), f64(bias), before[:rows, :n], True)
     check_product(torch.from_numpy(after[:rows, :n]), v, mag, torch.bfloat16, 1)
     after[:rows, :n] = before[:rows, :n]
     np.testing.assert_array_equal(after, before)
+
+
+def test_offsets_past_32_bits():
+    """Codes, outputs and tokens of more than 2^31 bytes or elements: the last rows against the definitions."""
+    rng = np.random.default_rng(11)
+    # codes: 1100000 rows of 2048
+    rows, k, n = 1100000, 2048, 20
+    a = torch.randint(-128, 128, (rows, k), dtype=torch.int8, device="cuda")
+    _, _, w, sw, bias, _ = make(rng, 1, k, n, 1, torch.float32, False)
+    sa = torch.rand(rows, device="cuda")
+    got = int8.matmul(a, sa, int8.pack_codes(w, sw), bias=bias, dtype=torch.float32)
+    v, mag = ref_product(a[-300:].cpu().numpy(), sa[-300:].cpu().numpy(), w.cpu().numpy().reshape(n, 1, k), sw.cpu().numpy(), f64(bias), None, False)
+    check_product(got[-300:], v, mag, torch.float32, 1)
+    # the same codes as 2200 images of 20 x 25 pixels
+    _, _, w, sw, bias, _ = make(rng, 1, k, n, 9, torch.float32, False)
+    got = int8.conv3x3(a.view(2200, 20, 25, k), sa.view(2200, 20, 25), int8.pack_codes(w, sw), bias=bias, dtype=torch.float16)
+    v, mag = ref_product(a[-500:].cpu().numpy(), sa[-500:].cpu().numpy(), w.cpu().numpy().reshape(n, 9, k), sw.cpu().numpy(), f64(bias), None, False,
+                         (1, 20, 25))
+    check_product(got[-1], v, mag, torch.float16, 9)
+    # tokens: more than 2^31 bfloat16 numbers
+    del a, got
+    x = torch.randn(1100000, k, dtype=torch.bfloat16, device="cuda")
+    codes, scales = int8.quantize_tokens(x)
+    q, s = ref_quantize(f64(x[-50:]))
+    np.testing.assert_array_equal(codes[-50:].cpu().numpy(), q)
+    np.testing.assert_array_equal(scales[-50:].cpu().numpy(), s)
+    del x, codes
+    # outputs: 70000 x 32768
+    a, sa, w, sw, bias, _ = make(rng, 70000, 64, 32768, 1, torch.bfloat16, False)
+    got = int8.matmul(a, sa, int8.pack_codes(w, sw), bias=bias)
+    v, mag = ref_product(a[-40:].cpu().numpy(), sa[-40:].cpu().numpy(), w.cpu().numpy().reshape(32768, 1, 64), sw.cpu().numpy(), f64(bias), None, False)
+    check_product(got[-40:], v, mag, torch.bfloat16, 1)
+
+
+def test_quantize_more_tokens_than_a_launch_has_threads_for():
+    """2^29 + 77 tokens of one channel, codes one byte apart: the scale is |x| / 127 and the code 127 with x's sign."""
+    rows = (1 << 29) + 77
+    x = torch.randn(rows, dtype=torch.float16, device="cuda")
+    codes, scales = torch.zeros(rows, dtype=torch.int8, device="cuda"), torch.zeros(rows, device="cuda")
+    _hip.check(_hip.lib().rcv_i8_quantize_tokens(x.data_ptr(), 1, 1, None, 0, 0, _hip.RCV_F16, rows, codes.data_ptr(), 1, scales.data_ptr(),
+                                                 _hip.current_stream()))
+    for part in (slice(0, 1000), slice((1 << 29) - 1000, rows)):
+        q, s = ref_quantize(f64(x[part])[:, None])
+        np.testing.assert_array_equal(codes[part].cpu().numpy(), q[:, 0])
+        np.testing.assert_array_equal(scales[part].cpu().numpy(), s)
+    assert bool(((codes != 0) == (x != 0)).all())
+
+
+def test_two_streams_and_two_graphs_at_once():
+    """Products whose sums are divided (they use a workspace): on two streams at once, and from two graphs replayed in turn and together."""
+    rng = np.random.default_rng(3)
+    calls, want = [], []
+    for rows, k, n in ((200, 8200, 900), (70, 20000, 1300)):
+        a, sa, w, sw, bias, _ = make(rng, rows, k, n, 1, torch.float32, False)
+        weight = int8.pack_codes(w, sw)
+        assert _hip.load_library().rcv_i8_matmul_workspace_bytes(rows, k, n) > 0
+        calls.append(lambda a=a, sa=sa, weight=weight, bias=bias: int8.matmul(a, sa, weight, bias=bias, dtype=torch.float32))
+        want.append(calls[-1]())
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        got = [[], []]
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i] = [calls[i]() for _ in range(4)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(calls[i]())
+        graphs.append(g)
+    for turn in range(4):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for i in (0, 1) if turn % 2 else (1, 0):
+            with torch.cuda.stream(streams[i if turn > 1 else 0]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(outs[i], want[i]) for i in range(2))
+        assert torch.equal(calls[0](), want[0])
 
 
 def test_nan_tokens_poison_their_window_and_nothing_else():

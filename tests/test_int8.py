@@ -113,6 +113,24 @@ def test_weight_refusals():
         int8.pack_codes(torch.ones(1, 131072, dtype=torch.int8), torch.ones(1))
 
 
+def test_packed_weight_refusals():
+    """A weight put together by hand has to have the layout that the kernels read."""
+    good = int8.pack_codes(torch.ones(8, 40, dtype=torch.int8), torch.ones(8))
+    int8.Int8Weight(good.codes, good.scales, 40)
+    for codes, scales, channels in ((good.codes.float(), good.scales, 40), (good.codes[:, 0], good.scales, 40), (good.codes, good.scales, 129),
+                                    (good.codes, good.scales, 0), (good.codes[:, :, :64], good.scales, 40),
+                                    (good.codes.expand(8, 2, 128).contiguous(), good.scales, 40), (good.codes.expand(8, 9, 128), good.scales, 40),
+                                    (good.codes[:0], good.scales[:0], 40), (good.codes, good.scales[:7], 40), (good.codes, good.scales.double(), 40),
+                                    (good.codes, torch.ones(16)[::2], 40)):
+        with pytest.raises(ValueError):
+            int8.Int8Weight(codes, scales, channels)
+
+
+def test_more_rows_than_a_launch_has_threads_for_are_refused():
+    assert _call("rcv_i8_matmul", _args(rows=(1 << 30) + 1)) == _hip.RCV_E_TOO_LARGE
+    assert _call("rcv_i8_conv3x3", _args(rows=12 << 28)) == _hip.RCV_E_TOO_LARGE
+
+
 def test_no_cpu_fallback():
     if torch.cuda.is_available():
         pytest.skip("GPU present")
