@@ -27,15 +27,17 @@ template <typename T> __device__ __forceinline__ T as_out(float v) { return (T)v
 // quantiser
 // ---------------------------------------------------------------------------------------------
 
-// round-half-even(x / s) of the exact quotient, s a normal number, |x| <= 127 s (1 + 2^-24): the product with 1/s is off by less
-// than one step, and the remainder x - q s is exact in one fma (it has no more significant bits than x and s share), so comparing
-// it with s / 2 settles the neighbours of a half.
-__device__ __forceinline__ int quantize_exact(float x, float s, float inv)
+// The code of x under scale s (a normal number, |x| <= 127 s (1 + 2^-24)): round-half-even(x / s) of the exact quotient in the low byte.
+// `m` is x / s + MAGIC rounded, MAGIC = 1.5 * 2^23: the whole number in its low bits is off by at most one where the quotient is near a
+// half.  The remainder x - q s is exact in one fma (it has no more significant bits than x and s share); a whole number gives way to its
+// neighbour where twice the remainder is above s, an odd one already at s.
+constexpr float MAGIC = 12582912.f;
+__device__ __forceinline__ unsigned settle(float x, float s, float m)
 {
-    float q = rintf(x * inv);
-    const float r2 = 2.f * fmaf(-q, s, x), m = fabsf(r2);
-    if (m > s || (m == s && ((int)q & 1))) q += copysignf(1.f, r2);
-    return (int)q;
+    const float q = m - MAGIC, r = fmaf(-q, s, x), r2 = r + r;
+    const unsigned bits = __float_as_uint(m);
+    const float limit = __uint_as_float(__float_as_uint(s) - (bits & 1u));
+    return bits + (fabsf(r2) > limit ? (unsigned)((__float_as_int(r2) >> 31) | 1) : 0u);
 }
 
 // The bits of |x| as a 32-bit number that orders like |x|, NaNs above the infinity.
@@ -63,26 +65,33 @@ __device__ __forceinline__ float token_scale(unsigned bits)
     return s < 0x1p-126f ? 0.f : s;
 }
 
-// Codes of sixteen channels.  x / s + 1.5 * 2^23 in one fma leaves the code, rounded half to even, in the low byte; with 1/s rounded
-// the quotient is off by at most 127 * 2^-23 < 2^-15, so only a remainder within 2^-15 of a half can be wrong, and those (few)
-// chunks are done again exactly.
+// Codes of sixteen channels.  With 1/s rounded the quotient is off by at most 127 * 2^-23 < 2^-15, so only a remainder within 2^-15 of a
+// half can lead to the wrong whole number: for float32 and float16 the chunks that hold one (6 % and about 20 % of the waves) are settled
+// in a second pass.  Among bfloat16's few numbers one in some hundreds is half the row's largest, whose quotient is 63.5 but for the
+// rounding of s: nearly every wave would take the second pass, so each code is settled at once.
 template <typename T> __device__ __forceinline__ uint4 quantize_chunk(const T *v, float s, float inv)
 {
-    constexpr float MAGIC = 12582912.f;
+    constexpr bool AT_ONCE = std::is_same<T, __bf16>::value;
     unsigned w[4];
     float d = 0.f;
+    auto put = [&](int e, unsigned bits) {
+        const unsigned b = bits & 255u;
+        w[e >> 2] = e & 3 ? w[e >> 2] | b << (8 * (e & 3)) : b;
+    };
 #pragma unroll
     for (int e = 0; e < 16; e++) {
         const float x = as_f32(v[e]), m = fmaf(x, inv, MAGIC);
-        d = fmaxf(d, fabsf(fmaf(x, inv, MAGIC - m)));
-        const unsigned b = __float_as_uint(m) & 255u;
-        w[e >> 2] = e & 3 ? w[e >> 2] | b << (8 * (e & 3)) : b;
+        if constexpr (AT_ONCE) put(e, settle(x, s, m));
+        else {
+            d = fmaxf(d, fabsf(fmaf(x, inv, MAGIC - m)));
+            put(e, __float_as_uint(m));
+        }
     }
-    if (d > 0.5f - 0x1p-15f) {
+    if (!AT_ONCE && d > 0.5f - 0x1p-15f) {
 #pragma unroll
         for (int e = 0; e < 16; e++) {
-            const unsigned b = (unsigned)quantize_exact(as_f32(v[e]), s, inv) & 255u;
-            w[e >> 2] = e & 3 ? w[e >> 2] | b << (8 * (e & 3)) : b;
+            const float x = as_f32(v[e]);
+            put(e, settle(x, s, fmaf(x, inv, MAGIC)));
         }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
@@ -97,7 +106,11 @@ __device__ __forceinline__ void store_chunk(int8_t *codes, uint4 w, int C, int c
     }
 }
 
-// L lanes per token, NV chunks of sixteen channels a lane: one pass, the token stays in registers.
+// L lanes per token, NV chunks of sixteen channels a lane: one pass, the token stays in registers.  Bound by memory: 63600 bfloat16 tokens
+// of 2048 channels 77 us and float16 ones 72 us (391 MB: 5.1 and 5.4 TB/s, a copy reaches 5.1), float32 119 us (652 MB: 5.5 TB/s).  The
+// fewest lanes that hold the token are taken: idle lanes cost instructions (us, bfloat16: 100000 x 128 with 8 / 16 / 32 lanes 10.0 / 15.1 /
+// 25.7, 300000 x 32 with 2 / 4 / 8 lanes 8.1 / 12.0 / 19.7, 50000 x 512 with 32 / 64 lanes 16.1 / 26.4), and twice the chunks in half the
+// lanes gains nothing (100000 x 256 with 8 lanes of two chunks 17.0, 16 of one 16.1) and lengthens small calls (300 x 1024 with 32 lanes of two 4.0, 64 of one 3.4).
 template <typename T, int L, int NV>
 __global__ __launch_bounds__(256) void k_i8_quantize(const T *x0, long long pitch0, int c0, const T *x1, long long pitch1, int c1,
                                                      long long rows, int8_t *codes, long long codes_pitch, float *scales, bool aligned)
@@ -782,7 +795,10 @@ int launch_quantize(const void *x0_, long long pitch0, int c0, const void *x1_, 
             hipLaunchKernelGGL((k_i8_quantize<T, L, NV>), dim3((unsigned)((n + 256 / L - 1) / (256 / L))), dim3(256), 0, st, a, pitch0, c0, b, \
                                pitch1, c1, n, q, codes_pitch, s, aligned);                                                        \
         });
+    RCV_I8_Q(1, 1)
+    RCV_I8_Q(2, 1)
     RCV_I8_Q(4, 1)
+    RCV_I8_Q(8, 1)
     RCV_I8_Q(16, 1)
     RCV_I8_Q(32, 1)
     RCV_I8_Q(64, 1)
@@ -837,7 +853,7 @@ Plan plan_product(long long rows, int K, int Cout, int taps, int groups)
             const long long wgs = tile_count(rows, Cout, groups, 128, 128);
             if (taps == 9) pl.splits = wgs * 9 <= 288 ? 9 : wgs * 3 <= 288 ? 3 : 1;
             else
-                while (wgs * pl.splits * 2 <= 288 && steps >= pl.splits * 2 * 16) pl.splits *= 2;
+                while (wgs * pl.splits * 2 <= (pl.splits == 1 ? 288 : 160) && steps >= pl.splits * 2 * 16) pl.splits *= 2;
         }
     }
     if (pl.splits > 1) pl.bytes = (size_t)pl.splits * groups * rows * ((Cout + 3) / 4) * 16;
