@@ -106,65 +106,88 @@ __device__ __forceinline__ void store_chunk(int8_t *codes, uint4 w, int C, int c
     }
 }
 
-// L lanes per token, NV chunks of sixteen channels a lane: one pass, the token stays in registers.  Bound by memory: 63600 bfloat16 tokens
-// of 2048 channels 77 us and float16 ones 72 us (391 MB: 5.1 and 5.4 TB/s, a copy reaches 5.1), float32 119 us (652 MB: 5.5 TB/s).  The
-// fewest lanes that hold the token are taken: idle lanes cost instructions (us, bfloat16: 100000 x 128 with 8 / 16 / 32 lanes 10.0 / 15.1 /
-// 25.7, 300000 x 32 with 2 / 4 / 8 lanes 8.1 / 12.0 / 19.7, 50000 x 512 with 32 / 64 lanes 16.1 / 26.4), and twice the chunks in half the
-// lanes gains nothing (100000 x 256 with 8 lanes of two chunks 17.0, 16 of one 16.1) and lengthens small calls (300 x 1024 with 32 lanes of two 4.0, 64 of one 3.4).
-template <typename T, int L, int NV>
+// L lanes per token, sixteen channels a lane: one pass, the token stays in registers.  The fewest lanes that hold the token are taken, as
+// idle lanes cost instructions (us, bfloat16: 100000 x 128 with 8 / 16 / 32 lanes 10.0 / 15.1 / 25.7, 300000 x 32 with 2 / 4 / 8 lanes
+// 8.1 / 12.0 / 19.7, 50000 x 512 with 32 / 64 lanes 16.1 / 26.4); twice the channels in half the lanes gains nothing (100000 x 256 with 8
+// lanes 17.0, 16 lanes 16.1) and lengthens small calls (300 x 1024 with 32 lanes 4.0, 64 lanes 3.4).
+template <typename T, int L>
 __global__ __launch_bounds__(256) void k_i8_quantize(const T *x0, long long pitch0, int c0, const T *x1, long long pitch1, int c1,
                                                      long long rows, int8_t *codes, long long codes_pitch, float *scales, bool aligned)
 {
     const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / L;
-    const int lane = threadIdx.x % L, C = c0 + c1;
+    const int lane = threadIdx.x % L, C = c0 + c1, c = lane * 16;
     if (row >= rows) return;
-    T v[NV][16];
+    T v[16];
     unsigned top = 0;
+    if (c < C) load_chunk(v, x0 + row * pitch0, c0, x1 + row * pitch1, C, c);
+    else
+        for (int e = 0; e < 16; e++) v[e] = (T)0.f;
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int c = (i * L + lane) * 16;
-        if (c < C) load_chunk(v[i], x0 + row * pitch0, c0, x1 + row * pitch1, C, c);
-        else
-            for (int e = 0; e < 16; e++) v[i][e] = (T)0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < NV; i++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) top = max(top, magnitude_bits(v[i][e]));
+    for (int e = 0; e < 16; e++) top = max(top, magnitude_bits(v[e]));
 #pragma unroll
     for (int o = L / 2; o; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
     const float s = token_scale(top), inv = s > 0.f ? 1.f / s : 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int c = (i * L + lane) * 16;
-        if (c < C) store_chunk(codes + row * codes_pitch, s > 0.f ? quantize_chunk(v[i], s, inv) : make_uint4(0u, 0u, 0u, 0u), C, c, aligned);
-    }
+    if (c < C) store_chunk(codes + row * codes_pitch, s > 0.f ? quantize_chunk(v, s, inv) : make_uint4(0u, 0u, 0u, 0u), C, c, aligned);
     if (lane == 0) scales[row] = s;
 }
 
-// A workgroup per token of any length: the token is read twice, the second time from the caches.
-template <typename T>
-__global__ __launch_bounds__(1024) void k_i8_quantize_long(const T *x0, long long pitch0, int c0, const T *x1, long long pitch1, int c1,
-                                                           int8_t *codes, long long codes_pitch, float *scales, bool aligned)
+// A workgroup of NW waves per token, NV chunks of sixteen channels a lane in registers.  NV = 0: a token of any length, read twice (the
+// second time from the caches).
+// Bound by memory: 63600 tokens of 2048 channels, in bfloat16 75 us and in float16 67 us (391 MB: 5.2 and 5.9 TB/s, a copy reaches 5.1), in
+// float32 115 us (652 MB: 5.7 TB/s).  A single token of 4096 channels: 3 us.  Shapes, us for bfloat16 / float16 / float32: 63600 x 2048 with 128
+// lanes of one chunk 75 / 67 / 115, 64 of two 73 / 71 / 119, and a single token 3.1 / 2.8 / 2.8 against 3.7 / 3.3 / 3.3; 30000 x 4096 with
+// 256 of one 68 / 65 / 107, 128 of two 69 / 68 / 112, 64 of four 75 / 70 / 114; 10000 x 5000 with 256 of two 32 / 29 / 40, 512 of one
+// 36 / 34 / 38; 8192 x 16384 with 1024 of one 77 / 72 / 117, read twice 90 / 83 / 150.
+template <typename T, int NW, int NV>
+__global__ __launch_bounds__(64 * NW) void k_i8_quantize_wide(const T *x0, long long pitch0, int c0, const T *x1, long long pitch1, int c1,
+                                                              int8_t *codes, long long codes_pitch, float *scales, bool aligned)
 {
-    __shared__ unsigned tops[16];
+    constexpr int LANES = 64 * NW;
+    __shared__ unsigned tops[NW];
     const long long row = blockIdx.x;
-    const int C = c0 + c1;
-    T v[16];
+    const int C = c0 + c1, first = threadIdx.x * 16;
+    const T *t0 = x0 + row * pitch0, *t1 = x1 + row * pitch1;
+    T v[NV ? NV : 1][16];
     unsigned top = 0;
-    for (int c = threadIdx.x * 16; c < C; c += 1024 * 16) {
-        load_chunk(v, x0 + row * pitch0, c0, x1 + row * pitch1, C, c);
+    auto scan = [&](const T *u) {
 #pragma unroll
-        for (int e = 0; e < 16; e++) top = max(top, magnitude_bits(v[e]));
+        for (int e = 0; e < 16; e++) top = max(top, magnitude_bits(u[e]));
+    };
+    if constexpr (NV == 0) {
+        for (int c = first; c < C; c += LANES * 16) {
+            load_chunk(v[0], t0, c0, t1, C, c);
+            scan(v[0]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = i * LANES * 16 + first;
+            if (c < C) load_chunk(v[i], t0, c0, t1, C, c);
+            else
+                for (int e = 0; e < 16; e++) v[i][e] = (T)0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; i++) scan(v[i]);
     }
+#pragma unroll
     for (int o = 32; o; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
     if (threadIdx.x % 64 == 0) tops[threadIdx.x / 64] = top;
     __syncthreads();
-    for (int w = 0; w < 16; w++) top = max(top, tops[w]);
+#pragma unroll
+    for (int w = 0; w < NW; w++) top = max(top, tops[w]);
     const float s = token_scale(top), inv = s > 0.f ? 1.f / s : 0.f;
-    for (int c = threadIdx.x * 16; c < C; c += 1024 * 16) {
-        load_chunk(v, x0 + row * pitch0, c0, x1 + row * pitch1, C, c);
-        store_chunk(codes + row * codes_pitch, s > 0.f ? quantize_chunk(v, s, inv) : make_uint4(0u, 0u, 0u, 0u), C, c, aligned);
+    auto store = [&](const T *u, int c) {
+        store_chunk(codes + row * codes_pitch, s > 0.f ? quantize_chunk(u, s, inv) : make_uint4(0u, 0u, 0u, 0u), C, c, aligned);
+    };
+    if constexpr (NV == 0) {
+        for (int c = first; c < C; c += LANES * 16) {
+            load_chunk(v[0], t0, c0, t1, C, c);
+            store(v[0], c);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+            if (i * LANES * 16 + first < C) store(v[i], i * LANES * 16 + first);
     }
     if (threadIdx.x == 0) scales[row] = s;
 }
@@ -789,25 +812,33 @@ int launch_quantize(const void *x0_, long long pitch0, int c0, const void *x1_, 
         }
         return RCV_OK;
     };
-#define RCV_I8_Q(L, NV)                                                                                                           \
-    if (C <= L * NV * 16)                                                                                                         \
+#define RCV_I8_Q(L)                                                                                                               \
+    if (C <= L * 16)                                                                                                              \
         return in_parts((1LL << 31) / L, [&](const T *a, const T *b, long long n, int8_t *q, float *s) {                          \
-            hipLaunchKernelGGL((k_i8_quantize<T, L, NV>), dim3((unsigned)((n + 256 / L - 1) / (256 / L))), dim3(256), 0, st, a, pitch0, c0, b, \
+            hipLaunchKernelGGL((k_i8_quantize<T, L>), dim3((unsigned)((n + 256 / L - 1) / (256 / L))), dim3(256), 0, st, a, pitch0, c0, b, \
                                pitch1, c1, n, q, codes_pitch, s, aligned);                                                        \
         });
-    RCV_I8_Q(1, 1)
+    RCV_I8_Q(1)
+    RCV_I8_Q(2)
+    RCV_I8_Q(4)
+    RCV_I8_Q(8)
+    RCV_I8_Q(16)
+    RCV_I8_Q(32)
+    RCV_I8_Q(64)
+#undef RCV_I8_Q
+#define RCV_I8_Q(NW, NV)                                                                                                          \
+    if (!NV || C <= 64 * NW * NV * 16)                                                                                             \
+        return in_parts((1LL << 31) / (64 * NW), [&](const T *a, const T *b, long long n, int8_t *q, float *s) {                  \
+            hipLaunchKernelGGL((k_i8_quantize_wide<T, NW, NV>), dim3((unsigned)n), dim3(64 * NW), 0, st, a, pitch0, c0, b, pitch1, c1, q, \
+                               codes_pitch, s, aligned);                                                                          \
+        });
     RCV_I8_Q(2, 1)
     RCV_I8_Q(4, 1)
-    RCV_I8_Q(8, 1)
+    RCV_I8_Q(4, 2)
     RCV_I8_Q(16, 1)
-    RCV_I8_Q(32, 1)
-    RCV_I8_Q(64, 1)
-    RCV_I8_Q(64, 2)
-    RCV_I8_Q(64, 4)
+    RCV_I8_Q(16, 0)
 #undef RCV_I8_Q
-    return in_parts((1LL << 31) / 1024, [&](const T *a, const T *b, long long n, int8_t *q, float *s) {
-        hipLaunchKernelGGL((k_i8_quantize_long<T>), dim3((unsigned)n), dim3(1024), 0, st, a, pitch0, c0, b, pitch1, c1, q, codes_pitch, s, aligned);
-    });
+    return RCV_E_TOO_LARGE;
 }
 
 // Lets `kernel` use more than the default 64 KB of LDS on the current device, once (ready: one bit per device).

@@ -92,7 +92,8 @@ def make(rng, rows, k, n, taps, dtype, residual, pitch=None):
     return a, sa, w, sw, bias, res
 
 
-QUANT = [(1, 1), (1, 4096), (3, 16), (5, 333), (67, 64), (130, 128), (9, 2048), (4, 5000), (2, 40000)]
+QUANT = [(1, 1), (1, 4096), (3, 16), (5, 333), (67, 64), (130, 128), (9, 2048), (4, 5000), (2, 40000),
+         (70, 30), (71, 100), (40, 1500), (33, 3000), (3, 8192), (4, 10000), (2, 131071)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
@@ -304,17 +305,24 @@ def test_offsets_past_32_bits():
 
 
 def test_quantize_more_tokens_than_a_launch_has_threads_for():
-    """2^29 + 77 tokens of one channel, codes one byte apart: the scale is |x| / 127 and the code 127 with x's sign."""
-    rows = (1 << 29) + 77
-    x = torch.randn(rows, dtype=torch.float16, device="cuda")
-    codes, scales = torch.zeros(rows, dtype=torch.int8, device="cuda"), torch.zeros(rows, device="cuda")
-    _hip.check(_hip.lib().rcv_i8_quantize_tokens(x.data_ptr(), 1, 1, None, 0, 0, _hip.RCV_F16, rows, codes.data_ptr(), 1, scales.data_ptr(),
+    """2^30 + 77 tokens of 17 channels: the first rows, those about 2^30 and the last; zeros between."""
+    rows, c = (1 << 30) + 77, 17
+    x = torch.zeros(rows, c, dtype=torch.float16, device="cuda")
+    parts = [slice(0, 500), slice((1 << 30) - 500, rows)]
+    for part in parts:
+        x[part].normal_()
+    codes, scales = torch.full((rows, c), 5, dtype=torch.int8, device="cuda"), torch.full((rows,), -1.0, device="cuda")
+    _hip.check(_hip.lib().rcv_i8_quantize_tokens(x.data_ptr(), c, c, None, 0, 0, _hip.RCV_F16, rows, codes.data_ptr(), c, scales.data_ptr(),
                                                  _hip.current_stream()))
-    for part in (slice(0, 1000), slice((1 << 29) - 1000, rows)):
-        q, s = ref_quantize(f64(x[part])[:, None])
-        np.testing.assert_array_equal(codes[part].cpu().numpy(), q[:, 0])
+    for part in parts:
+        q, s = ref_quantize(f64(x[part]))
+        np.testing.assert_array_equal(codes[part].cpu().numpy(), q)
         np.testing.assert_array_equal(scales[part].cpu().numpy(), s)
-    assert bool(((codes != 0) == (x != 0)).all())
+    for start in range(500, (1 << 30) - 500, 1 << 28):
+        part = slice(start, min(start + (1 << 28), (1 << 30) - 500))
+        assert int(scales[part].count_nonzero()) == 0 and int(codes[part].count_nonzero()) == 0
+    del x, codes, scales
+    torch.cuda.empty_cache()
 
 
 def test_two_streams_and_two_graphs_at_once():
