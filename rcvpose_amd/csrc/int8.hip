@@ -459,6 +459,26 @@ template <int I, int N, typename F> __device__ __forceinline__ void for_each(F &
     }
 }
 
+// r[i] of the four 16-lane rows k <-> r[k] of row i: a 4 x 4 transposition between registers and rows of lanes.
+__device__ __forceinline__ void transpose_rows(float &r0, float &r1, float &r2, float &r3)
+{
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+    auto swap32 = [](float &a, float &b) {  // the upper half of a <-> the lower half of b
+        const u32x2 v = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+        a = __uint_as_float(v[0]);
+        b = __uint_as_float(v[1]);
+    };
+    auto swap16 = [](float &a, float &b) {  // the odd rows of a <-> the even rows of b
+        const u32x2 v = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+        a = __uint_as_float(v[0]);
+        b = __uint_as_float(v[1]);
+    };
+    swap32(r0, r2);
+    swap32(r1, r3);
+    swap16(r0, r1);
+    swap16(r2, r3);
+}
+
 template <int TAPS_, int WT_, int WC_, int TT_, int CT_, int NA_, int NB_, bool SPLIT_ = false> struct TileShape {
     static constexpr bool SPLIT = SPLIT_;  // the sum may be divided over workgroups
     static constexpr int TAPS = TAPS_, WT = WT_, WC = WC_, TT = TT_, CT = CT_, NA = NA_, NB = NB_;
@@ -467,7 +487,8 @@ template <int TAPS_, int WT_, int WC_, int TT_, int CT_, int NA_, int NB_, bool 
     static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;      // pieces (8 rows) of a wave per step
     static constexpr int A_BYTES = BM * KB, B_BYTES = BN * KB, B_RING = NA * A_BYTES, TABLE = B_RING + NB * B_BYTES;
     static constexpr int LDS = TABLE + (TAPS == 9 ? 9 * BM * 4 : 0);
-    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && LDS <= 160 * 1024 && NA >= 3 && NB >= 2 && NB <= NA && BM <= 64 * NW, "tile plan");
+    static constexpr bool STAGED = TT * CT <= 8;                  // the epilogue goes through LDS
+    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && LDS <= 160 * 1024 && NA >= 3 && NB >= 2 && NB <= NA && BM <= 64 * NW && CT == 4, "tile plan");
     // Pieces in order of issue, per step kt: the tokens of step kt + NA - 1 in its first half, the weights of step kt + NB in its second.
     // Half-way through step kt everything of step kt + 1 has to be there: what may still be on its way was issued later.
     static constexpr int LATE = NB == NA ? (NA - 2) * (PA + PB) : (NB - 2) * (PA + PB) + PA;
@@ -478,7 +499,7 @@ template <int TAPS_, int WT_, int WC_, int TT_, int CT_, int NA_, int NB_, bool 
 // chunks of a row are permuted (chunk ^= row bits) on the way in, so that the sixteen rows of a fragment read fall on all banks.
 // One barrier per step, half-way: before it a wave has read the step's last fragments, behind it the next step's first are there.
 //
-// TAPS = 9 walks tap by tap; after every tap the integer sums are scaled into `sum`.
+// TAPS = 9 walks tap by tap.  The integer sums of a tap are scaled into `sum` between the first products of the next.
 //
 // gridDim.y > 1 divides the sum: a workgroup takes its share of the channels (TAPS = 1) or of the taps and leaves raw sums in `partial`
 // [split][group][rows][quads of channels] for k_i8_finish.
@@ -528,24 +549,23 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_i8_tile(const I8Product p, in
         const unsigned cols = (x > 0 ? 1u : 0u) | 2u | (x + 1 < W ? 4u : 0u);
         return (y > 0 ? cols : 0u) | cols << 3 | (y + 1 < H ? cols << 6 : 0u);
     };
-    // What the epilogue needs, requested first: the scales of this lane's tokens, the scales and biases of the V channels it will finish.
+    // What a staged epilogue needs, requested first: the scales of this lane's tokens, the scales and biases of the V channels it will finish.
     constexpr int V = 16 / sizeof(T), CPR = BN / V;
-    constexpr bool LATE_SCALES = TT * CT > 16 && TAPS == 1;  // (no registers to keep them over the loop)
     const int c = tid % CPR, n = n0 + c * V;
     float sa[TT] = {};
     typename Row<float, V>::Vec sw = {}, bias = {};
-    auto load_scales = [&]() {
-        if constexpr (!S::SPLIT) {
+    auto load_token_scales = [&]() {
 #pragma unroll
-            for (int j = 0; j < TT; j++) {
-                const int row = wt * TT * 16 + j * 16 + r16;
-                sa[j] = TAPS == 1 && row < left ? cs[m0 + row] : 0.f;
-            }
-            sw = load_row<float, V>(p.weight_scales + (long long)g * p.weight_scale_gs + n, n, p.Cout);
-            if (p.bias) bias = load_row<float, V>(p.bias + (long long)g * p.bias_gs + n, n, p.Cout);
+        for (int j = 0; j < TT; j++) {
+            const int row = (wt * TT + j) * 16 + r16;
+            sa[j] = row < left ? cs[m0 + row] : 0.f;
         }
     };
-    if constexpr (!LATE_SCALES) load_scales();
+    if constexpr (S::STAGED && !S::SPLIT) {
+        if constexpr (TAPS == 1) load_token_scales();
+        sw = load_row<float, V>(p.weight_scales + (long long)g * p.weight_scale_gs + n, n, p.Cout);
+        if (p.bias) bias = load_row<float, V>(p.bias + (long long)g * p.bias_gs + n, n, p.Cout);
+    }
 
     // this lane's part of the pieces: row lane / 8 of the piece, 16-byte slot lane % 8
     auto chunk_of = [&](int row, int slot) { return slot ^ ((row >> 1) & 7); };
@@ -631,8 +651,19 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_i8_tile(const I8Product p, in
         if (step(ib)) b_tap();
     };
 
+    // [9][BM] in LDS: the scale under which a token's tap enters, 0 outside the image (there the offset is out of range and the load gives 0).
+    // Requested before the pieces, so that storing them waits for no piece.
+    float tap_scale[9] = {};
+    if constexpr (TAPS == 9) {
+        const __amdgpu_buffer_rsrc_t view_s = view((const int8_t *)(cs + (m0 - W - 1)), (p.rows - m0 + W + 1) * 4);
+        const unsigned ok = tid < BM ? taps_inside(tid) : 0u;
+#pragma unroll
+        for (int t = 0; t < 9; t++)
+            tap_scale[t] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(view_s, (ok >> t) & 1u ? (tid + (t / 3) * W + t % 3) * 4 : OOB, 0, 0));
+    }
     a_view();
     b_view();
+#pragma unroll
     for (int s = 0; s < S::NA - 1; s++) {  // tokens of steps 0 .. NA - 2 and weights of steps 0 .. NB - 1 in the order of the loop
         for_each<0, PA>(a_piece);
         a_end();
@@ -646,20 +677,12 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_i8_tile(const I8Product p, in
         b_end();
     }
 
-    float *sa_tab = (float *)(smem + S::TABLE);  // [9][BM]: the scale under which a token's tap enters, 0 outside the image
-    if constexpr (TAPS == 9) {
-        // (nine loads in flight: outside the image the offset is out of range and the load gives 0)
-        const __amdgpu_buffer_rsrc_t view_s = view((const int8_t *)(cs + (m0 - W - 1)), (p.rows - m0 + W + 1) * 4);
+    float *sa_tab = (float *)(smem + S::TABLE);
+    if constexpr (TAPS == 9)
         if (tid < BM) {
-            const unsigned ok = taps_inside(tid);
-            float v[9];
 #pragma unroll
-            for (int t = 0; t < 9; t++)
-                v[t] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(view_s, (ok >> t) & 1u ? (tid + (t / 3) * W + t % 3) * 4 : OOB, 0, 0));
-#pragma unroll
-            for (int t = 0; t < 9; t++) sa_tab[t * BM + tid] = v[t];
+            for (int t = 0; t < 9; t++) sa_tab[t * BM + tid] = tap_scale[t];
         }
-    }
 
     i32x4 acc[CT][TT];
     f32x4 sum[TAPS == 9 ? CT : 1][TAPS == 9 ? TT : 1];
@@ -670,6 +693,7 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_i8_tile(const I8Product p, in
             acc[i][j] = i32x4{0, 0, 0, 0};
             if constexpr (TAPS == 9) sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
+    float sc[TT] = {};  // TAPS = 9: the scales of the tap whose sums are in acc
     i32x4 tf[2][TT], wf[2][CT];
     const int t_row = (wt * TT * 16 + r16) * KB, w_row = S::B_RING + (wc * CT * 16 + r16) * KB;
     int a_stage = 0, b_stage = 0;  // byte offsets of the stages being read
@@ -680,23 +704,35 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_i8_tile(const I8Product p, in
     };
     // all products of fragment set f; meanwhile the other set is read from `half` of the current stages and N pieces are issued
     constexpr int NM = TT * CT, NF = TT + CT, SEG = NM / 4, RSEG = SEG / 2;  // (the reads go into the first half: they are back before the barrier)
-    auto multiply = [&](auto ff, int half, auto count, auto &&piece) {
+    auto multiply = [&](auto ff, int half, auto count, auto &&piece, auto first) {
         constexpr int f = decltype(ff)::value, n = decltype(count)::value;
         for_each<0, SEG>([&](auto ss) {
             constexpr int s = decltype(ss)::value;
 #pragma unroll
             for (int q = 0; q < NF; q++) if (q * RSEG / NF == s) read(1 - f, half, q);
             for_each<s * n / SEG, (s + 1) * n / SEG>(piece);
-            // (reads, half of the products, a piece, the others: with its addresses computed under the first two products a piece costs less
-            // than in the compiler's order: 518 against 526 us for the window over 53 images of 30 x 40, 2048 -> 512 channels)
-            __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-            __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+            if constexpr (decltype(first)::value) {
 #pragma unroll
-            for (int e = s * 4; e < s * 4 + 4; e++) {
-                const int i = e / TT, j = e % TT;
-                acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[f][i], tf[f][j], acc[i][j], 0, 0, 0);
+                for (int e = s * 4; e < s * 4 + 4; e++) {
+                    const int i = e / TT, j = e % TT;
+#pragma unroll
+                    for (int q = 0; q < 4; q++) sum[i][j][q] = fmaf((float)acc[i][j][q], sc[j], sum[i][j][q]);
+                    asm volatile("" : "+v"(sum[i][j]));  // (here: put off, it would keep the old sums in registers of their own)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[f][i], tf[f][j], i32x4{0, 0, 0, 0}, 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            } else {
+                // (reads, half of the products, a piece, the others: with its addresses computed under the first two products a piece costs
+                // less than in the compiler's order: 518 against 526 us for the window over 53 images of 30 x 40, 2048 -> 512 channels)
+                __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+#pragma unroll
+                for (int e = s * 4; e < s * 4 + 4; e++) {
+                    const int i = e / TT, j = e % TT;
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[f][i], tf[f][j], acc[i][j], 0, 0, 0);
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
         });
@@ -709,90 +745,150 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_i8_tile(const I8Product p, in
     step_barrier<S::LATE + PB>();
 #pragma unroll
     for (int q = 0; q < NF; q++) read(0, 0, q);
+    auto finish_step = [&]() {
+        a_end();
+        step_barrier<S::LATE>();  // the next step is here; nobody reads the current one any more
+        a_stage = a_stage == (S::NA - 1) * S::A_BYTES ? 0 : a_stage + S::A_BYTES;
+        b_stage = b_stage == (S::NB - 1) * S::B_BYTES ? 0 : b_stage + S::B_BYTES;
+        multiply(c1, 0, pb, b_piece, std::false_type{});
+        b_end();
+    };
     for (int tap = tap0; tap < tap1; tap++) {
-        for (int k = klo; k < khi; k += KB) {
-            multiply(c0, 1, pa, a_piece);
-            a_end();
-            step_barrier<S::LATE>();  // the next step is here; nobody reads the current one any more
-            a_stage = a_stage == (S::NA - 1) * S::A_BYTES ? 0 : a_stage + S::A_BYTES;
-            b_stage = b_stage == (S::NB - 1) * S::B_BYTES ? 0 : b_stage + S::B_BYTES;
-            multiply(c1, 0, pb, b_piece);
-            b_end();
-        }
+        int k = klo;
         if constexpr (TAPS == 9) {
+            multiply(c0, 1, pa, a_piece, std::true_type{});
 #pragma unroll
-            for (int j = 0; j < TT; j++) {
-                const float sa = sa_tab[tap * BM + wt * TT * 16 + j * 16 + r16];
-#pragma unroll
-                for (int i = 0; i < CT; i++) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) sum[i][j][e] = fmaf((float)acc[i][j][e], sa, sum[i][j][e]);
-                    acc[i][j] = i32x4{0, 0, 0, 0};
-                }
-            }
+            for (int j = 0; j < TT; j++) sc[j] = sa_tab[tap * BM + wt * TT * 16 + j * 16 + r16];
+            finish_step();
+            k += KB;
+        }
+        for (; k < khi; k += KB) {
+            multiply(c0, 1, pa, a_piece, std::false_type{});
+            finish_step();
         }
     }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // (the last pieces: zeros nobody reads)
-
-    if constexpr (LATE_SCALES) load_scales();
-    // Epilogue: the scaled sums go through LDS, so that rows leave (and the residual's rows come) in whole lines.
-    constexpr int SROW = BN + 4, ROUND = 64 * S::NW / CPR;
-    static_assert(BM * SROW * 4 <= S::LDS || S::TAPS == 1, "the tile fits");
-    constexpr int PARTS = BM * SROW * 4 <= S::LDS ? 1 : 2, PROWS = BM / PARTS;
-    float *stage = (float *)smem;
+    if constexpr (TAPS == 9) {
+#pragma unroll
+        for (int i = 0; i < CT; i++)
+#pragma unroll
+            for (int j = 0; j < TT; j++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) sum[i][j][q] = fmaf((float)acc[i][j][q], sc[j], sum[i][j][q]);
+    }
     float vmax = 0.f;
+    if constexpr (S::STAGED) {
+        // The scaled sums go through LDS, so that rows leave (and the residual's rows come) in whole lines.
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // (the last pieces: zeros nobody reads)
+        constexpr int SROW = BN + 4, ROUND = 64 * S::NW / CPR;
+        static_assert(BM * SROW * 4 <= S::LDS, "the tile fits");
+        float *stage = (float *)smem;
+        __syncthreads();  // the rings have been read
 #pragma unroll
-    for (int part = 0; part < PARTS; part++) {
-        __syncthreads();  // the ring (the part before) has been read
-        if (PARTS == 1 || wt * TT * 16 / PROWS == part) {
+        for (int i = 0; i < CT; i++) {
+            const int col = (wc * CT + i) * 16 + kq * 4;
 #pragma unroll
-            for (int i = 0; i < CT; i++) {
-                const int col = (wc * CT + i) * 16 + kq * 4;
+            for (int j = 0; j < TT; j++) {
+                f32x4 v;
 #pragma unroll
-                for (int j = 0; j < TT; j++) {
-                    const int row = wt * TT * 16 + j * 16 + r16;
-                    f32x4 v;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        if constexpr (TAPS == 9) v[e] = sum[i][j][e];
-                        else v[e] = S::SPLIT ? __int_as_float(acc[i][j][e]) : (float)acc[i][j][e] * sa[j];
-                    }
-                    *(f32x4 *)(stage + (row - part * PROWS) * SROW + col) = v;
+                for (int e = 0; e < 4; e++) {
+                    if constexpr (TAPS == 9) v[e] = sum[i][j][e];
+                    else v[e] = S::SPLIT ? __int_as_float(acc[i][j][e]) : (float)acc[i][j][e] * sa[j];
                 }
+                *(f32x4 *)(stage + ((wt * TT + j) * 16 + r16) * SROW + col) = v;
             }
         }
         __syncthreads();
         constexpr int AHEAD = 4;  // residual rows requested together
-        static_assert(PROWS % (ROUND * AHEAD) == 0, "whole rounds");
+        static_assert(BM % (ROUND * AHEAD) == 0, "whole rounds");
         if constexpr (S::SPLIT) {  // raw sums: float32 (TAPS = 9) or integers
             const long long quads = (p.Cout + 3) / 4;
-            for (int r = tid / (BN / 4); r < PROWS; r += 64 * S::NW / (BN / 4)) {
-                const int row = part * PROWS + r, col = tid % (BN / 4);
+            for (int row = tid / (BN / 4); row < BM; row += 64 * S::NW / (BN / 4)) {
+                const int col = tid % (BN / 4);
                 if (row < left && n0 + col * 4 < p.Cout)
-                    partial[(((long long)blockIdx.y * p.groups + g) * p.rows + m0 + row) * quads + n0 / 4 + col] = *(const f32x4 *)(stage + r * SROW + col * 4);
+                    partial[(((long long)blockIdx.y * p.groups + g) * p.rows + m0 + row) * quads + n0 / 4 + col] = *(const f32x4 *)(stage + row * SROW + col * 4);
             }
         } else if (n < p.Cout)
-            for (int r0 = tid / CPR; r0 < PROWS; r0 += ROUND * AHEAD) {
+            for (int r0 = tid / CPR; r0 < BM; r0 += ROUND * AHEAD) {
                 typename Row<T, V>::Vec res[AHEAD] = {};
                 if (p.residual) {
 #pragma unroll
                     for (int a = 0; a < AHEAD; a++) {
-                        const int row = part * PROWS + r0 + a * ROUND;
+                        const int row = r0 + a * ROUND;
                         if (row < left) res[a] = load_row<T, V>(residual_row<T>(p, g, m0 + row) + n, n, p.Cout);
                     }
                 }
 #pragma unroll
                 for (int a = 0; a < AHEAD; a++) {
-                    const int r = r0 + a * ROUND, row = part * PROWS + r;
+                    const int row = r0 + a * ROUND;
                     if (row >= left) continue;
                     float v[V];
 #pragma unroll
-                    for (int q = 0; q < V / 4; q++) *(f32x4 *)(v + 4 * q) = *(const f32x4 *)(stage + r * SROW + c * V + 4 * q);
+                    for (int q = 0; q < V / 4; q++) *(f32x4 *)(v + 4 * q) = *(const f32x4 *)(stage + row * SROW + c * V + 4 * q);
 #pragma unroll
                     for (int e = 0; e < V; e++) v[e] = fmaf(v[e], sw[e], bias[e]);
                     vmax = fmaxf(vmax, finish_row<T, V>(p, g, m0 + row, n, v, res[a]));
                 }
             }
+    } else {
+        // Every wave finishes its part from registers.  A lane takes N consecutive channels of a token: 16-bit rows leave as whole 128-byte lines
+        // after a 4 x 4 transposition between a lane's four tiles and the four rows of lanes, float32 rows as 64-byte pieces of their own.
+        // (Against the way through LDS: 16384 x 1024 -> 4096 108 -> 101 us, the window over 53 images of 30 x 40, 2048 -> 512 channels 499 ->
+        // 492 us; the small tiles lose by it, 16384 x 256 -> 2048 30.2 -> 31.3 us.)
+        constexpr int N = sizeof(T) == 2 ? 16 : 4, Q = 16 / N;
+        auto channel = [&](int q) { return n0 + wc * CT * 16 + (N == 16 ? kq * 16 : q * 16 + kq * 4); };
+        typename Row<float, N>::Vec ws[Q] = {}, bs[Q] = {};
+#pragma unroll
+        for (int q = 0; q < Q; q++) {
+            const int nq = channel(q);
+            if (nq < p.Cout) {
+                ws[q] = load_row<float, N>(p.weight_scales + (long long)g * p.weight_scale_gs + nq, nq, p.Cout);
+                if (p.bias) bs[q] = load_row<float, N>(p.bias + (long long)g * p.bias_gs + nq, nq, p.Cout);
+            }
+        }
+        if constexpr (TAPS == 1) load_token_scales();
+        constexpr int AHEAD = 4;  // residual rows requested together
+        static_assert(TT % AHEAD == 0, "whole rounds");
+#pragma unroll
+        for (int j0 = 0; j0 < TT; j0 += AHEAD) {
+            typename Row<T, N>::Vec res[AHEAD][Q] = {};
+            if (p.residual) {
+#pragma unroll
+                for (int a = 0; a < AHEAD; a++) {
+                    const int row = (wt * TT + j0 + a) * 16 + r16;
+#pragma unroll
+                    for (int q = 0; q < Q; q++) {
+                        const int nq = channel(q);
+                        if (row < left && nq < p.Cout) res[a][q] = load_row<T, N>(residual_row<T>(p, g, m0 + row) + nq, nq, p.Cout);
+                    }
+                }
+            }
+#pragma unroll
+            for (int a = 0; a < AHEAD; a++) {
+                const int j = j0 + a, row = (wt * TT + j) * 16 + r16;
+                float v[CT][4];
+#pragma unroll
+                for (int i = 0; i < CT; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        if constexpr (TAPS == 9) v[i][e] = sum[i][j][e];
+                        else v[i][e] = (float)acc[i][j][e] * sa[j];
+                    }
+                if constexpr (N == 16) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) transpose_rows(v[0][e], v[1][e], v[2][e], v[3][e]);
+                }
+#pragma unroll
+                for (int q = 0; q < Q; q++) {
+                    const int nq = channel(q);
+                    if (row >= left || nq >= p.Cout) continue;
+                    float o[N];
+#pragma unroll
+                    for (int e = 0; e < N; e++) o[e] = fmaf(v[q + e / 4][e % 4], ws[q][e], bs[q][e]);
+                    vmax = fmaxf(vmax, finish_row<T, N>(p, g, m0 + row, nq, o, res[a][q]));
+                }
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // (the last pieces: zeros nobody reads)
     }
     report_range<T>(p, vmax);
 }
