@@ -953,34 +953,64 @@ struct Plan {
     enum Kind { WIDE, TALL, SQUARE, NARROW, DIRECT } kind;
     int splits;
     size_t bytes;  // of partial sums
+    bool wide_direct;  // DIRECT: two 16-channel tiles a workgroup
 };
 
-long long tile_count(long long rows, int Cout, int groups, int bm, int bn) { return ((rows + bm - 1) / bm) * ((Cout + bn - 1) / bn) * groups; }
-
+// The times beside the rules are microseconds of one call in a graph, bfloat16 out; M x K -> N for a product, images x height x width, K -> N
+// for a window.
 Plan plan_product(long long rows, int K, int Cout, int taps, int groups)
 {
-    Plan pl{Plan::SQUARE, 1, 0};
+    Plan pl{Plan::SQUARE, 1, 0, false};
     const int steps = taps * ((K + 127) / 128);
-    const long long small = tile_count(rows, Cout, groups, 64, 16);
-    if (rows <= 64 || (small <= (taps == 9 ? 480 : 320) && small * 80 * taps * i8_kp(K) <= 60000000)) {
+    auto tiles = [&](int bm, int bn) { return ((rows + bm - 1) / bm) * ((Cout + bn - 1) / bn) * groups; };
+
+    // Straight from memory, where the tiles are few and read few bytes of tokens (each reads its own: with all weights read once, 4 x 8192 ->
+    // 32768 takes 45, through LDS 50; 8 rows 51 / 51, 16 rows 64 / 54).  Direct / through LDS: 300 x 2048 -> 512 7.8 / 10.5,
+    // 128 x 1024 -> 1024 5.4 / 8.0, 32 x 4096 -> 4096 9.0 / 11.2, 64 x 4096 -> 4096 12.9 / 12.4, 64 x 8192 -> 8192 26 / 20; more than 64
+    // rows: 512 x 1024 -> 1024 8.3 / 8.1, 1000 x 2048 -> 1000 17 / 12, short sums 391 x 291 -> 1136 4.9 / 7.1, 603 x 532 -> 1994 10.6 / 8.3;
+    // windows: 3 x 37 x 53, 96 -> 80 10.9 / 13.1, 1 x 60 x 80, 64 -> 64 9.7 / 12.9, 1 x 60 x 80, 128 -> 128 18.2 / 12.6,
+    // 1 x 15 x 20, 1024 -> 256 16.8 / 14.1.
+    const long long small = tiles(64, 16);
+    // (two 16-channel tiles per workgroup share the tokens once all CUs are busy: 32 x 1024 -> 8192 5.2 / 6.1, 64 x 2048 -> 8192 9.8 / 12.5,
+    // but 32 x 4096 -> 4096 10.6 / 8.9)
+    pl.wide_direct = taps == 1 && rows > 16 && small >= 512;
+    const long long token_bytes = (pl.wide_direct ? tiles(64, 32) : small) * std::min(rows, 64LL) * taps * i8_kp(K);
+    const bool few = taps == 9 ? small <= 480 : small <= 320 || (small <= 640 && token_bytes <= 16000000);
+    if (rows <= 4 || (token_bytes <= 60000000 && (rows <= 64 || few))) {
         pl.kind = Plan::DIRECT;
-        const long long wgs = small;
-        while (wgs * pl.splits * 2 <= 256 && steps >= pl.splits * 2 * 16) pl.splits *= 2;  // (at least four 64-channel steps a wave)
+        // Workgroups divide a long sum while CUs are free.  In 1 / 2 / 4 / 8 parts: 1 x 16384 -> 512 11.7 / 9.4 / 7.7 / 7.5, 1 x 4096 -> 512
+        // 5.3 / 6.1 / 6.2 / 7.0, 1 x 8192 -> 64 7.3 / 7.0 / 6.8, 45 x 2343 -> 758 5.9 / 7.1, 64 x 4096 -> 512 12.0 / 9.9 / 8.4, 1 x 8 x 8, 2048 -> 256 39 / 24 / 17 / 14, 1 x 5 x 7, 512 -> 64
+        // 10.7 / 10.1 / 8.9 / 9.2, 3 x 26 x 8, 147 -> 30 7.0 / 8.2.
+        const int part = taps == 9 ? 9 : rows > 32 ? 8 : 16;
+        if (steps >= (taps == 9 ? 36 : rows > 16 ? 24 : 64))
+            while (pl.splits < 8 && small * pl.splits * 2 <= 256 && steps >= pl.splits * 2 * part) pl.splits *= 2;
     } else {
         // rounds of the chip's 256 CUs times the relative time of a tile
-        auto cost = [&](int bm, int bn, double w) { return (double)((tile_count(rows, Cout, groups, bm, bn) + 255) / 256) * w; };
+        auto cost = [&](int bm, int bn, double w) { return (double)((tiles(bm, bn) + 255) / 256) * w; };
         if (taps == 1) {
-            const long long wide = tile_count(rows, Cout, groups, 256, 256);
+            // 256 x 256 tiles move half the bytes of 128 x 128 ones, but need a long sum behind their start and end, and full rounds.
+            // 256 / 128: 16384 x 8192 -> 4096 391 / 509, 16384 x 2048 -> 4096 135 / 160, x 1024 101 / 102, x 512 85 / 74; rounds
+            // filled to 0.81: 3328 x 4096 -> 4096 61 / 68, 0.69: 2816 rows 54 / 56, 0.56: 4608 rows 105 / 90, 0.50: 2048 rows 53 / 39.
+            const long long wide = tiles(256, 256);
             if (K >= 1024 && wide * 4 >= 3 * ((wide + 255) / 256 * 256)) pl.kind = Plan::WIDE;
         } else if (Cout <= 64) {
+            // 256 x 64 tiles against 128 x 128 ones that are half empty: 16 x 240 x 320, 192 -> 64 336 / 618, 3 x 120 x 160, 256 -> 64 19 / 33;
+            // where each needs one round the times are equal (1 x 120 x 160 17.2 / 17.1) and the smaller tiles can be divided by taps.
             if (cost(256, 64, 0.66) <= cost(128, 128, 0.62)) pl.kind = Plan::NARROW;
         } else if (cost(256, 128, 1.0) <= cost(128, 128, 0.62))
+            // 256 x 128 / 128 x 128: 53 x 30 x 40, 2048 -> 512 551 / 663, 8 x 60 x 80, 128 -> 128 20 / 25; one round of either:
+            // 12 x 15 x 20, 2048 -> 1024 106 / 83
             pl.kind = Plan::TALL;
-        if (pl.kind == Plan::SQUARE && steps >= 48) {
-            const long long wgs = tile_count(rows, Cout, groups, 128, 128);
-            if (taps == 9) pl.splits = wgs * 9 <= 288 ? 9 : wgs * 3 <= 288 ? 3 : 1;
-            else
-                while (wgs * pl.splits * 2 <= (pl.splits == 1 ? 288 : 160) && steps >= pl.splits * 2 * 16) pl.splits *= 2;
+        if (pl.kind == Plan::SQUARE) {
+            // Few tiles of a long sum: workgroups divide it while the CUs hold them at once.  In 1 / 3 / 9 parts (taps): 1 x 15 x 20,
+            // 2048 -> 1024 67 / 30 / 23, 1 x 30 x 40, 2048 -> 512 68 / 32 / 33, 1 x 60 x 80, 1024 -> 256 39 / 27 / 44, 512 -> 256 23 / 24 / 35,
+            // 128 -> 256 13 / 21 / 37, 1 x 30 x 40, 512 -> 512 23 / 18 / 26, 256 -> 512 16 / 16 / 26; in 1 / 2 / 4 parts (channels):
+            // 512 x 8192 -> 1024 35 / 21 / 17, 512 x 8192 -> 2048 35 / 24 / 27, 1024 x 8192 -> 2048 37 / 34 / 44, 64 x 4096 -> 4096
+            // 16 / 13 / 12, 512 x 4096 -> 2048 17 / 20 / 20.
+            const long long wgs = tiles(128, 128);
+            if (taps == 9) pl.splits = wgs <= 32 && steps >= 36 ? 9 : wgs <= 96 && steps >= (wgs <= 48 ? 18 : 40) ? 3 : 1;
+            else if (steps >= (wgs <= 40 ? 32 : 48))
+                while (wgs * pl.splits * 2 <= (pl.splits == 1 ? 288 : 160) && steps >= pl.splits * 2 * 8) pl.splits *= 2;
         }
     }
     if (pl.splits > 1) pl.bytes = (size_t)pl.splits * groups * rows * ((Cout + 3) / 4) * 16;
@@ -1029,6 +1059,8 @@ template <typename T, int TAPS> int launch_taps(const I8Product &p, const Plan &
 {
     if (pl.kind == Plan::DIRECT) {
         if (p.rows <= 16) return launch_direct<T, TAPS, 1, 1, TAPS == 1 ? 4 : 2>(p, pl, ws, st);
+        if constexpr (TAPS == 1)
+            if (pl.wide_direct) return p.rows <= 32 ? launch_direct<T, 1, 2, 2, 2>(p, pl, ws, st) : launch_direct<T, 1, 4, 2, 2>(p, pl, ws, st);
         if (p.rows <= 32) return launch_direct<T, TAPS, 2, 1, TAPS == 1 ? 4 : 2>(p, pl, ws, st);
         return launch_direct<T, TAPS, 4, 1, 2>(p, pl, ws, st);
     }
