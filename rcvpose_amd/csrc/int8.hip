@@ -264,6 +264,8 @@ template <typename T> __device__ __forceinline__ void report_range(const I8Produ
 // every wave multiplies its own run of 64-channel steps with nothing shared, D steps of loads in flight, so a short call is a few
 // memory round trips long.  The waves' sums meet in LDS and are added in order; with gridDim.y > 1 they go to `partial`
 // [split][group][rows][quads] and k_i8_finish adds them in order.  Integer sums (TAPS = 1) are exact whatever the order.
+// Bound by memory where one token meets many weights (1 x 8192 -> 32768: 268 MB in 43 us, 6.2 TB/s), by the depth of the loads in flight
+// where there is little to read (300 x 2048 -> 512: 7.8 us, of which a launch is 2.8).
 template <typename T, int TAPS, int TT, int CT, int NW, int D>
 __global__ __launch_bounds__(64 * NW, 2) void k_i8_direct(const I8Product p, int tiles_n, f32x4 *partial)
 {
@@ -500,6 +502,11 @@ template <int TAPS_, int WT_, int WC_, int TT_, int CT_, int NA_, int NB_, bool 
 // One barrier per step, half-way: before it a wave has read the step's last fragments, behind it the next step's first are there.
 //
 // TAPS = 9 walks tap by tap.  The integer sums of a tap are scaled into `sum` between the first products of the next.
+//
+// What bounds it: at long sums the card's power (16384 x 8192 -> 8192: 828 us, 2.66 POP/s, matrix units 0.66 busy at 1.7 to 1.8 GHz; a loop
+// of the same instructions on registers 3.4 to 3.95) and, for windows, the copies into LDS (53 x 30 x 40, 2048 -> 512: 502 us, 2.4
+// POP/s; without its products 377 us, without its copies 339).  At short ones a tile's start and end: 2 and 5 us beside 0.7 us a step (24 x
+// 120 x 160, 512 -> 128: 314 us, 1.7 POP/s).  Fewer bytes per product are what helps, hence tiles as large as the registers allow.
 //
 // gridDim.y > 1 divides the sum: a workgroup takes its share of the channels (TAPS = 1) or of the taps and leaves raw sums in `partial`
 // [split][group][rows][quads of channels] for k_i8_finish.
