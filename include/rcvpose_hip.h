@@ -452,7 +452,9 @@ int rcv_i8_quantize_tokens(const void *x0_dev, long long pitch0, int c0, const v
  *
  * rcv_i8_matmul: one tap, m(tap) = m.  rcv_i8_conv3x3: the nine taps of a 3x3 window with zero padding and stride 1 over images of
  * height x width tokens (rows = images * height * width, row-major).  Sums within a tap are exact 32-bit integers, taps are added
- * in float32 in a fixed order, the result is rounded once to out_dtype: two calls give the same bits.  ReLU keeps a NaN.
+ * in float32 in an order that the sizes alone decide, the result is rounded once to out_dtype: two calls of one size give the same bits.
+ * (rcv_i8_matmul gives a row the same bits whatever the other sizes; a window among more or fewer images may differ in its float32
+ * sum's last bits.)  ReLU keeps a NaN.
  *   codes       rows codes_pitch bytes apart; 16-byte aligned, codes_pitch a multiple of 16, and the last row readable up to
  *               channels rounded up to a multiple of 16 (what lies there has no influence); -128 is allowed
  *   weights     [out_channels][taps][channels rounded up to a multiple of 128], 16-byte aligned, zeros behind `channels`

@@ -478,7 +478,8 @@ class FcnEngine:
     the split product as one block-scaled fp6 matrix instruction (engine option 11, q6_wanted): -18 % on those launches, -3 % on
     the forward, for 2-3x the map error (worst network of the bench 3.4e-5 -> 7.8e-5 of the 1e-4 tolerance: r05 measurement).
     int8 (bf16 / fp16; default off): True or a regex over convolution names -- those stride-1 convolutions run on 8-bit integers with one
-    scale per pixel and output channel (engine option 16, int8_wanted).
+    scale per pixel and output channel (engine option 16, int8_wanted).  Their maps may differ between batch sizes by the rounding of a
+    float32 sum (the nine taps of a window are added in an order that depends on the batch).
     """
 
     def __init__(self, state_dicts, H, W, dtype="bf16", device="cuda", reuse_slots=True, arch="dense", q6=False, int8=False):

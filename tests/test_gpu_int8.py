@@ -272,6 +272,19 @@ def test_output_rows_at_a_pitch(rows, n, pitch):
     np.testing.assert_array_equal(after, before)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_token_has_the_same_product_in_any_batch(dtype):
+    """One token, sixteen, a few hundred and many run on different kernels; the integer sums are exact, so a row's bits are the same."""
+    rng = np.random.default_rng(17)
+    for k, n in ((1100, 520), (8200, 140)):
+        a, sa, w, sw, bias, res = make(rng, 9000, k, n, 1, dtype, True)
+        weight = int8.pack_codes(w, sw)
+        full = int8.matmul(a, sa, weight, bias=bias, residual=res, relu=True, dtype=dtype)
+        for start, stop in ((0, 1), (8999, 9000), (100, 116), (200, 264), (300, 500), (1000, 3000)):
+            part = slice(start, stop)
+            assert torch.equal(int8.matmul(a[part], sa[part], weight, bias=bias, residual=res[part], relu=True, dtype=dtype), full[part])
+
+
 def test_offsets_past_32_bits():
     """Codes, outputs and tokens of more than 2^31 bytes or elements: the last rows against the definitions."""
     rng = np.random.default_rng(11)

@@ -192,3 +192,11 @@ def test_model_takes_int8_with_16_bit_types_only():
         with pytest.raises(ValueError):
             m.set_compute_dtype(name, int8=True)
     assert m.compute_dtype == "fp16"
+
+
+def test_main_takes_int8():
+    from rcvpose_amd import main
+
+    assert main.build_parser().parse_args([]).int8 is False
+    opts = main.build_parser().parse_args(["--dtype", "bf16", "--int8", "true"])
+    assert opts.int8 is True and opts.dtype == "bf16"
