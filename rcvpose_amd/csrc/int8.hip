@@ -265,9 +265,10 @@ template <typename T> __device__ __forceinline__ void report_range(const I8Produ
 // memory round trips long.  The waves' sums meet in LDS and are added in order; with gridDim.y > 1 they go to `partial`
 // [split][group][rows][quads] and k_i8_finish adds them in order.  Integer sums (TAPS = 1) are exact whatever the order.
 // Bound by memory where one token meets many weights (1 x 8192 -> 32768: 268 MB in 43 us, 6.2 TB/s), by the depth of the loads in flight
-// where there is little to read (300 x 2048 -> 512: 7.8 us, of which a launch is 2.8).
+// where there is little to read (300 x 2048 -> 512: 7.8 us, of which a launch is 2.8).  Two workgroups on a CU count for more than deeper
+// loads: windows of 64 tokens with D = 1 in 96 registers against D = 2 in 136, 3 x 37 x 53, 96 -> 80 8.8 / 10.9 us.
 template <typename T, int TAPS, int TT, int CT, int NW, int D>
-__global__ __launch_bounds__(64 * NW, 2) void k_i8_direct(const I8Product p, int tiles_n, f32x4 *partial)
+__global__ __launch_bounds__(64 * NW, CT == 1 ? 4 : 2) void k_i8_direct(const I8Product p, int tiles_n, f32x4 *partial)
 {
     constexpr int OOB = (int)0x80000000, TILE_N = CT * 16, ROW = TILE_N + 4;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -413,15 +414,23 @@ template <typename T, int TAPS> __global__ __launch_bounds__(256) void k_i8_fini
     const long long m = q / quads, stride = (long long)p.groups * p.rows * quads;
     const f32x4 *at = partial + (long long)g * p.rows * quads + q;
     f32x4 v = at[0];
-    if constexpr (TAPS == 9) {
-        for (int s = 1; s < splits; s++) {
-            const f32x4 o = at[s * stride];
+    constexpr int AHEAD = 8;  // parts requested together
+    for (int s0 = 1; s0 < splits; s0 += AHEAD) {
+        f32x4 o[AHEAD];
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] += o[e];
+        for (int s = 0; s < AHEAD; s++) o[s] = s0 + s < splits ? at[(s0 + s) * stride] : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < AHEAD; s++) {
+            if (s0 + s >= splits) continue;
+            if constexpr (TAPS == 9) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] += o[s][e];
+            } else
+                v = __builtin_bit_cast(f32x4, __builtin_bit_cast(i32x4, v) + __builtin_bit_cast(i32x4, o[s]));
         }
-    } else {
-        i32x4 t = __builtin_bit_cast(i32x4, v);
-        for (int s = 1; s < splits; s++) t += __builtin_bit_cast(i32x4, at[s * stride]);
+    }
+    if constexpr (TAPS == 1) {
+        const i32x4 t = __builtin_bit_cast(i32x4, v);
         const float sa = p.code_scales[(long long)g * p.code_gs + m];
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = (float)t[e] * sa;
@@ -975,22 +984,26 @@ Plan plan_product(long long rows, int K, int Cout, int taps, int groups)
     // 32768 takes 45, through LDS 50; 8 rows 51 / 51, 16 rows 64 / 54).  Direct / through LDS: 300 x 2048 -> 512 7.8 / 10.5,
     // 128 x 1024 -> 1024 5.4 / 8.0, 32 x 4096 -> 4096 9.0 / 11.2, 64 x 4096 -> 4096 12.9 / 12.4, 64 x 8192 -> 8192 26 / 20; more than 64
     // rows: 512 x 1024 -> 1024 8.3 / 8.1, 1000 x 2048 -> 1000 17 / 12, short sums 391 x 291 -> 1136 4.9 / 7.1, 603 x 532 -> 1994 10.6 / 8.3;
-    // windows: 3 x 37 x 53, 96 -> 80 10.9 / 13.1, 1 x 60 x 80, 64 -> 64 9.7 / 12.9, 1 x 60 x 80, 128 -> 128 18.2 / 12.6,
-    // 1 x 15 x 20, 1024 -> 256 16.8 / 14.1.
+    // windows: 3 x 37 x 53, 96 -> 80 8.8 / 13.1, 1 x 60 x 80, 64 -> 64 7.6 / 12.9, 64 -> 128 11.2 / 12.5, 128 -> 128 18.1 / 12.5,
+    // 1 x 13 x 58, 168 -> 467 9.7 / 14.2, 1 x 15 x 20, 1024 -> 256 17.2 / 13.2, 1 x 30 x 40, 512 -> 128 14.8 / 13.2.
     const long long small = tiles(64, 16);
     // (two 16-channel tiles per workgroup share the tokens once all CUs are busy: 32 x 1024 -> 8192 5.2 / 6.1, 64 x 2048 -> 8192 9.8 / 12.5,
     // but 32 x 4096 -> 4096 10.6 / 8.9)
     pl.wide_direct = taps == 1 && rows > 16 && small >= 512;
-    const long long token_bytes = (pl.wide_direct ? tiles(64, 32) : small) * std::min(rows, 64LL) * taps * i8_kp(K);
-    const bool few = taps == 9 ? small <= 480 : small <= 320 || (small <= 640 && token_bytes <= 16000000);
-    if (rows <= 4 || (token_bytes <= 60000000 && (rows <= 64 || few))) {
+    const long long token_bytes = (pl.wide_direct ? tiles(64, 32) : small) * std::min(rows, 64LL) * taps * ((K + 63) & ~63);
+    const bool few = small <= 320 || (small <= 640 && (taps == 9 || token_bytes <= 16000000));
+    // (windows whose rows lie whole cache lines apart read few of the cache's channels at a time: 1 x 30 x 40, 256 -> 256 15.2 / 14.0, but
+    // 3 x 21 x 18, 355 -> 208 9.7 / 14.4)
+    if (rows <= 4 || (token_bytes <= (taps == 9 && K % 128 == 0 ? 42000000 : 60000000) && (rows <= 64 || few))) {
         pl.kind = Plan::DIRECT;
         // Workgroups divide a long sum while CUs are free.  In 1 / 2 / 4 / 8 parts: 1 x 16384 -> 512 11.7 / 9.4 / 7.7 / 7.5, 1 x 4096 -> 512
-        // 5.3 / 6.1 / 6.2 / 7.0, 1 x 8192 -> 64 7.3 / 7.0 / 6.8, 45 x 2343 -> 758 5.9 / 7.1, 64 x 4096 -> 512 12.0 / 9.9 / 8.4, 1 x 8 x 8, 2048 -> 256 39 / 24 / 17 / 14, 1 x 5 x 7, 512 -> 64
-        // 10.7 / 10.1 / 8.9 / 9.2, 3 x 26 x 8, 147 -> 30 7.0 / 8.2.
-        const int part = taps == 9 ? 9 : rows > 32 ? 8 : 16;
-        if (steps >= (taps == 9 ? 36 : rows > 16 ? 24 : 64))
-            while (pl.splits < 8 && small * pl.splits * 2 <= 256 && steps >= pl.splits * 2 * part) pl.splits *= 2;
+        // 5.3 / 6.1 / 6.2 / 7.0, 1 x 8192 -> 64 7.3 / 7.0 / 6.8, 45 x 2343 -> 758 5.9 / 7.1, 64 x 4096 -> 512 12.0 / 9.9 / 8.4; windows
+        // 1 x 8 x 8, 2048 -> 256 39 / 24 / 17 / 14, 1 x 5 x 7, 512 -> 64 10.7 / 10.1 / 8.9 / 9.2, 1 x 20 x 5, 369 -> 112 11.2 / 10.9 / 9.3,
+        // 1 x 17 x 4, 288 -> 645 8.3 / 9.0, 3 x 26 x 8, 147 -> 30 7.0 / 8.2.
+        const int steps64 = taps * ((K + 63) / 64);
+        const int least = taps == 9 ? 54 : rows > 16 ? 47 : 128, part = taps == 9 ? 13 : rows > 32 ? 16 : rows > 16 ? 24 : 32;
+        if (steps64 >= least)
+            while (pl.splits < 8 && small * pl.splits * 2 <= 256 && steps64 >= pl.splits * 2 * part) pl.splits *= 2;
     } else {
         // rounds of the chip's 256 CUs times the relative time of a tile
         auto cost = [&](int bm, int bn, double w) { return (double)((tiles(bm, bn) + 255) / 256) * w; };
@@ -1010,14 +1023,15 @@ Plan plan_product(long long rows, int K, int Cout, int taps, int groups)
             pl.kind = Plan::TALL;
         if (pl.kind == Plan::SQUARE) {
             // Few tiles of a long sum: workgroups divide it while the CUs hold them at once.  In 1 / 3 / 9 parts (taps): 1 x 15 x 20,
-            // 2048 -> 1024 67 / 30 / 23, 1 x 30 x 40, 2048 -> 512 68 / 32 / 33, 1 x 60 x 80, 1024 -> 256 39 / 27 / 44, 512 -> 256 23 / 24 / 35,
-            // 128 -> 256 13 / 21 / 37, 1 x 30 x 40, 512 -> 512 23 / 18 / 26, 256 -> 512 16 / 16 / 26; in 1 / 2 / 4 parts (channels):
-            // 512 x 8192 -> 1024 35 / 21 / 17, 512 x 8192 -> 2048 35 / 24 / 27, 1024 x 8192 -> 2048 37 / 34 / 44, 64 x 4096 -> 4096
-            // 16 / 13 / 12, 512 x 4096 -> 2048 17 / 20 / 20.
+            // 2048 -> 1024 67 / 30 / 23, 1 x 30 x 40, 2048 -> 512 68 / 32 / 33, 3 x 28 x 43, 717 -> 127 30 / 19 / 24, 1 x 60 x 80,
+            // 1024 -> 256 39 / 27 / 44, 512 -> 256 23 / 24 / 35, 128 -> 256 13 / 21 / 37, 2 x 69 x 54, 488 -> 61 24 / 17 / 28,
+            // 3 x 29 x 33, 313 -> 452 20 / 30 / 38, 1 x 30 x 40, 512 -> 512 23 / 18 / 26, 256 -> 512 16 / 16 / 26; in 1 / 2 / 4 parts
+            // (channels): 697 x 2907 -> 493 14.2 / 13.2 / 12.6, 512 x 8192 -> 1024 35 / 21 / 17, 512 x 8192 -> 2048 35 / 24 / 27,
+            // 1024 x 8192 -> 2048 37 / 34 / 44, 64 x 4096 -> 4096 16 / 13 / 12, 512 x 4096 -> 2048 17 / 20 / 20.
             const long long wgs = tiles(128, 128);
-            if (taps == 9) pl.splits = wgs <= 32 && steps >= 36 ? 9 : wgs <= 96 && steps >= (wgs <= 48 ? 18 : 40) ? 3 : 1;
-            else if (steps >= (wgs <= 40 ? 32 : 48))
-                while (wgs * pl.splits * 2 <= (pl.splits == 1 ? 288 : 160) && steps >= pl.splits * 2 * 8) pl.splits *= 2;
+            if (taps == 9) pl.splits = wgs <= 24 && steps >= 36 ? 9 : wgs <= 85 && steps >= (wgs <= 48 ? 18 : 27) ? 3 : 1;
+            else if (steps >= (wgs <= 40 ? 20 : 48))
+                while (wgs * pl.splits * 2 <= (pl.splits == 1 ? 256 : 160) && steps >= pl.splits * 2 * 8) pl.splits *= 2;
         }
     }
     if (pl.splits > 1) pl.bytes = (size_t)pl.splits * groups * rows * ((Cout + 3) / 4) * 16;
@@ -1069,7 +1083,7 @@ template <typename T, int TAPS> int launch_taps(const I8Product &p, const Plan &
         if constexpr (TAPS == 1)
             if (pl.wide_direct) return p.rows <= 32 ? launch_direct<T, 1, 2, 2, 2>(p, pl, ws, st) : launch_direct<T, 1, 4, 2, 2>(p, pl, ws, st);
         if (p.rows <= 32) return launch_direct<T, TAPS, 2, 1, TAPS == 1 ? 4 : 2>(p, pl, ws, st);
-        return launch_direct<T, TAPS, 4, 1, 2>(p, pl, ws, st);
+        return launch_direct<T, TAPS, 4, 1, TAPS == 1 ? 2 : 1>(p, pl, ws, st);
     }
     if constexpr (TAPS == 1) {
         if (pl.kind == Plan::WIDE) return launch_tile<T, TileShape<1, 2, 4, 8, 4, 3, 2>>(p, pl, ws, st);
