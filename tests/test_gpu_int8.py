@@ -181,7 +181,9 @@ MATMUL = [(1, 1, 1), (1, 16, 5), (1, 4096, 300), (2, 131, 17), (3, 100, 33), (16
           (33000, 70, 40), (33023, 200, 9), (300, 150, 16500),
           (12300, 1030, 1025),
           # a long sum over few tiles, divided over workgroups
-          (200, 8200, 900), (70, 20000, 1300)]
+          (200, 8200, 900), (70, 20000, 1300),
+          # wide layers of few rows
+          (20, 200, 8300), (50, 130, 8200), (64, 8200, 4100), (3, 300, 20000)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
@@ -205,7 +207,7 @@ CONV = [(1, 1, 1, 16, 1), (1, 1, 9, 64, 32), (2, 9, 1, 48, 24), (2, 5, 7, 33, 19
         # enough output tiles for the large-product kernel
         (9, 61, 70, 33, 24), (7, 47, 101, 130, 120), (7, 47, 101, 40, 136), (33001, 1, 1, 20, 8), (1, 33000, 2, 16, 4),
         # a long sum over few tiles, divided by taps
-        (1, 13, 21, 1100, 300), (3, 40, 41, 700, 260)]
+        (1, 13, 21, 1100, 300), (3, 40, 41, 700, 260), (1, 30, 41, 300, 260), (2, 31, 33, 450, 61)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
@@ -270,6 +272,38 @@ def test_output_rows_at_a_pitch(rows, n, pitch):
     check_product(torch.from_numpy(after[:rows, :n]), v, mag, torch.bfloat16, 1)
     after[:rows, :n] = before[:rows, :n]
     np.testing.assert_array_equal(after, before)
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_sizes_drawn_at_random(seed):
+    """Sizes over the ranges in which the choice of kernel changes, every type, with and without bias, residual and ReLU."""
+    rng = np.random.default_rng(1000 + seed)
+    log = lambda lo, hi: int(round(lo * (hi / lo) ** rng.random()))
+    for _ in range(8):
+        dtype = [torch.float32, torch.bfloat16, torch.float16][rng.integers(3)]
+        residual, relu, with_bias = rng.random(3) < 0.5
+        taps = 1 if rng.random() < 0.5 else 9
+        if taps == 1:
+            m, k, n = log(1, 3000), log(1, 6000), log(1, 3000)
+            while m * k * n > 3e9:
+                m, n = max(1, m // 2), max(1, n // 2)
+            image = None
+        else:
+            b, h, wd, k, n = log(1, 4), log(1, 50), log(1, 50), log(1, 900), log(1, 400)
+            while b * h * wd * k * n > 3e8:
+                k, n = max(1, k // 2), max(1, n // 2)
+            m, image = b * h * wd, (b, h, wd)
+        a, sa, w, sw, bias, res = make(rng, m, k, n, taps, dtype, residual)
+        bias = bias if with_bias else None
+        weight = int8.pack_codes(w, sw)
+        if taps == 1:
+            got = int8.matmul(a, sa, weight, bias=bias, residual=res, relu=bool(relu), dtype=dtype)
+        else:
+            got = int8.conv3x3(a.unflatten(0, image), sa.view(image), weight, bias=bias, residual=None if res is None else res.view(image + (n,)),
+                               relu=bool(relu), dtype=dtype)
+        v, mag = ref_product(a.cpu().numpy(), sa.cpu().numpy(), w.cpu().numpy().reshape(n, taps, k), sw.cpu().numpy(),
+                             None if bias is None else f64(bias), None if res is None else f64(res), relu, image)
+        check_product(got, v, mag, dtype, taps)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
