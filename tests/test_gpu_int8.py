@@ -159,6 +159,26 @@ def test_quantize_extremes(dtype):
     assert np.isnan(s[3:6]).all() and np.isfinite(s[[0, 1, 2, 6, 7]]).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("c", [24, 100, 700, 1500, 5000])
+def test_quantize_at_every_magnitude(c, dtype):
+    """Rows from the smallest scale that counts to the largest numbers, with equal values, halves and powers of two of the row's largest among
+    them (quotients beside a half): every code and every scale exact."""
+    rng = np.random.default_rng(c)
+    lo, hi = (-16, 14) if dtype == torch.float16 else (-119, 126)
+    e = np.linspace(lo, hi, 200)
+    x = rng.standard_normal((200, c)) / 4
+    x[:, 0] = 1 + rng.random(200)
+    x[:, 1::5] = x[:, :1] * 2.0 ** -rng.integers(0, 9, size=(200, len(range(1, c, 5))))
+    x[:, 2::7] = x[:, :1] * (rng.integers(-127, 127, size=(200, len(range(2, c, 7)))) + 0.5) / 127
+    t = torch.from_numpy(x * 2.0 ** np.floor(e)[:, None]).to(dtype)
+    assert bool(torch.isfinite(t).all())
+    codes, scales = int8.quantize_tokens(t.cuda())
+    q, s = ref_quantize(f64(t))
+    np.testing.assert_array_equal(scales.cpu().numpy(), s)
+    np.testing.assert_array_equal(codes.cpu().numpy(), q)
+
+
 def test_quantize_leaves_the_pitch_alone():
     """Codes written into rows of a wider buffer: the bytes behind the last code and the rows behind the last token stay."""
     L = _hip.lib()
