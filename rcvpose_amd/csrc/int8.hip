@@ -966,7 +966,7 @@ int allow_lds(const void *kernel, int bytes, std::atomic<unsigned long long> &re
 
 // How a product runs.
 struct Plan {
-    enum Kind { WIDE, TALL, SQUARE, NARROW, DIRECT } kind;
+    enum Kind { WIDE /* SQUARE for short sums: wide_from */, TALL, SQUARE, NARROW, DIRECT } kind;
     int splits;
     size_t bytes;  // of partial sums
     bool wide_direct;  // DIRECT: two 16-channel tiles a workgroup
@@ -1008,11 +1008,11 @@ Plan plan_product(long long rows, int K, int Cout, int taps, int groups)
         // rounds of the chip's 256 CUs times the relative time of a tile
         auto cost = [&](int bm, int bn, double w) { return (double)((tiles(bm, bn) + 255) / 256) * w; };
         if (taps == 1) {
-            // 256 x 256 tiles move half the bytes of 128 x 128 ones, but need a long sum behind their start and end, and full rounds.
-            // 256 / 128: 16384 x 8192 -> 4096 391 / 509, 16384 x 2048 -> 4096 135 / 160, x 1024 101 / 102, x 512 85 / 74; rounds
-            // filled to 0.81: 3328 x 4096 -> 4096 61 / 68, 0.69: 2816 rows 54 / 56, 0.56: 4608 rows 105 / 90, 0.50: 2048 rows 53 / 39.
+            // 256 x 256 tiles move half the bytes of 128 x 128 ones, but need full rounds, and a long sum behind their start and end
+            // (wide_from).  256 / 128: 3328 x 4096 -> 4096 (rounds filled to 0.81) 55 / 64, 2816 rows (0.69) 51 / 52, 4608 rows (0.56)
+            // 98 / 81, 2048 rows (0.50) 49 / 36.
             const long long wide = tiles(256, 256);
-            if (K >= 1024 && wide * 4 >= 3 * ((wide + 255) / 256 * 256)) pl.kind = Plan::WIDE;
+            if (wide * 4 >= 3 * ((wide + 255) / 256 * 256)) pl.kind = Plan::WIDE;
         } else if (Cout <= 64) {
             // 256 x 64 tiles against 128 x 128 ones that are half empty: 16 x 240 x 320, 192 -> 64 336 / 618, 3 x 120 x 160, 256 -> 64 19 / 33;
             // where each needs one round the times are equal (1 x 120 x 160 17.2 / 17.1) and the smaller tiles can be divided by taps.
@@ -1076,6 +1076,16 @@ template <typename T, int TAPS, int TT, int CT, int D> int launch_direct(const I
     return partial ? launch_finish<T, TAPS>(p, pl, partial, st) : RCV_OK;
 }
 
+// The shortest sum for which 256 x 256 tiles pay.  256 / 128, us: 16384 rows -> 4096 channels of bfloat16, 512 69 / 71, 768 81 / 86, 1024 91 / 99, 2048
+// 135 / 153, 8192 400 / 483.  They finish from registers, with less to hide it behind: rows that start anywhere (4001 channels: 1024
+// 110 / 100, 1536 133 / 133, 2048 153 / 156) and residuals in pieces of lines (float32: 1024 196 / 153, 2048 239 / 206, 4096 326 / 331; bfloat16,
+// 4008 channels: 1024 126 / 115, 2048 168 / 170) need more.
+template <typename T> int wide_from(const I8Product &p)
+{
+    const long long pitch = p.out_pitch * (long long)sizeof(T);
+    return 768 + (sizeof(T) == 2 && pitch % 16 ? 1024 : 0) + (p.residual && (sizeof(T) == 4 || pitch % 128) ? 1792 : 0);
+}
+
 template <typename T, int TAPS> int launch_taps(const I8Product &p, const Plan &pl, void *ws, hipStream_t st)
 {
     if (pl.kind == Plan::DIRECT) {
@@ -1086,7 +1096,7 @@ template <typename T, int TAPS> int launch_taps(const I8Product &p, const Plan &
         return launch_direct<T, TAPS, 4, 1, TAPS == 1 ? 2 : 1>(p, pl, ws, st);
     }
     if constexpr (TAPS == 1) {
-        if (pl.kind == Plan::WIDE) return launch_tile<T, TileShape<1, 2, 4, 8, 4, 3, 2>>(p, pl, ws, st);
+        if (pl.kind == Plan::WIDE && p.K >= wide_from<T>(p)) return launch_tile<T, TileShape<1, 2, 4, 8, 4, 3, 2>>(p, pl, ws, st);
         if (pl.splits > 1) return launch_tile<T, TileShape<1, 4, 2, 2, 4, 5, 4, true>>(p, pl, ws, st);
         return launch_tile<T, TileShape<1, 4, 2, 2, 4, 3, 2>>(p, pl, ws, st);
     } else {

@@ -199,7 +199,7 @@ MATMUL = [(1, 1, 1), (1, 16, 5), (1, 4096, 300), (2, 131, 17), (3, 100, 33), (16
           (777, 1500, 333),
           # enough output tiles for the large-product kernel: many rows of few channels, few rows of many
           (33000, 70, 40), (33023, 200, 9), (300, 150, 16500),
-          (12300, 1030, 1025),
+          (12300, 1030, 1025), (12300, 1900, 1032), (12300, 3600, 1025),
           # a long sum over few tiles, divided over workgroups
           (200, 8200, 900), (70, 20000, 1300),
           # wide layers of few rows
@@ -272,7 +272,7 @@ def test_codes_inside_a_wider_matrix():
     check_product(got, v, mag, torch.float32, 1)
 
 
-@pytest.mark.parametrize("rows, n, pitch", [(5, 7, 12), (70, 64, 72), (300, 130, 131), (520, 128, 160), (2500, 260, 261), (20000, 1100, 1101)])
+@pytest.mark.parametrize("rows, n, pitch", [(5, 7, 12), (70, 64, 72), (300, 130, 131), (520, 128, 160), (2500, 260, 261), (20000, 1100, 1101), (20000, 1152, 1160)])
 def test_output_rows_at_a_pitch(rows, n, pitch):
     """The columns between two rows and the rows behind the last stay as they were, the residual may be the output itself."""
     rng = np.random.default_rng(rows)
