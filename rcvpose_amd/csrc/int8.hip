@@ -559,9 +559,12 @@ __global__ __launch_bounds__(64 * S::NW, 2) void k_i8_tile(const I8Product p, in
     }
     auto taps_inside = [&](int row) -> unsigned {
         if (row >= left) return 0u;
-        // (a product with the reciprocal, half a step up: the quotient is at most BM for W = 1 and 1 for the widest image, its error far
-        // below the half step's distance 1 / (2 W) to a whole number)
-        const int t = x0 + row, l = (int)(((float)t + 0.5f) * rw), x = t - l * W, yl = y0 + l, y = yl - (int)(((float)yl + 0.5f) * rh) * H;
+        // The image row l rows below the tile's first.  (A product with the reciprocal, half a step up: the quotient is at most BM for W = 1 and 1
+        // for the widest image of 65536 columns, its error far below the half step's distance 1 / (2 W) to a whole number.)
+        const int t = x0 + row, l = (int)(((float)t + 0.5f) * rw), x = t - l * W, yl = y0 + l;
+        // Heights have no such bound (float32 misplaces the last row of 6556022), but the tile reaches fewer than BM rows down: a taller image
+        // ends in it at most once, and for a lower one yl < 2 BM.
+        const int y = yl - (H >= BM ? (yl >= H ? H : 0) : (int)(((float)yl + 0.5f) * rh) * H);
         const unsigned cols = (x > 0 ? 1u : 0u) | 2u | (x + 1 < W ? 4u : 0u);
         return (y > 0 ? cols : 0u) | cols << 3 | (y + 1 < H ? cols << 6 : 0u);
     };

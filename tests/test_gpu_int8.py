@@ -513,3 +513,23 @@ def test_two_layers_as_a_network_runs_them():
     y = torch.nn.functional.conv2d(xf, w1.dequantize().double().cpu().permute(0, 3, 1, 2), b1.double().cpu(), padding=1).clamp_min(0)
     got = int8.conv3x3(q, s, w1, bias=b1, relu=True, dtype=torch.float32)
     assert float((got.cpu().double() - y.permute(0, 2, 3, 1)).abs().max()) <= 1e-5 * float(y.abs().max())
+
+
+@pytest.mark.parametrize("h, n", [(6556022, 4), (6556022, 72), (8399926, 4), (65537, 4), (257, 8)])
+def test_tall_images(h, n):
+    """Images of one column and of more rows than float32 numbers count exactly: the last rows of the first image and the first of the
+    second, whose windows end at the border between them (H = 6556022 is the smallest height whose last row a float32 quotient
+    misplaces, 8399926 the smallest whose next image's first row it does)."""
+    rng = np.random.default_rng(h)
+    c, dtype = 16, torch.bfloat16
+    images = 2 if h > 1000 else 4001  # (enough rows for the tiles through LDS)
+    a = torch.randint(-128, 128, (images * h, c), dtype=torch.int8, device="cuda")
+    sa = torch.rand(images * h, device="cuda") + 0.5
+    _, _, w, sw, bias, _ = make(rng, 1, c, n, 9, dtype, False)
+    got = int8.conv3x3(a.view(images, h, 1, c), sa.view(images, h, 1), int8.pack_codes(w, sw), bias=bias, dtype=dtype).view(images * h, n)
+    m = min(h - 1, 300)
+    for start, stop, first, last in ((h - m - 1, h, 1, m + 1), (h, h + m + 1, 0, m)):  # rows read, and those of them whose window is among them
+        part = slice(start, stop)
+        v, mag = ref_product(a[part].cpu().numpy(), sa[part].cpu().numpy(), w.cpu().numpy().reshape(n, 9, c), sw.cpu().numpy(), f64(bias), None, False,
+                             (1, m + 1, 1))
+        check_product(got[part][first:last], v[first:last], mag[first:last], dtype, 9)
