@@ -336,7 +336,7 @@ typedef struct rcv_fcn rcv_fcn; /* opaque engine handle */
 int rcv_fcn_create(const rcv_op *ops, int n_ops, int n_slots, const int64_t *slot_elems, int groups, int dtype,
                    const void *weights_dev, const float *bias_dev, rcv_fcn **out);
 void rcv_fcn_destroy(rcv_fcn *h);
-/* Activation workspace bytes for a batch of B images. */
+/* Activation workspace bytes for a batch of B images; never less for more images, so a workspace of the largest batch serves them all. */
 size_t rcv_fcn_workspace_bytes(const rcv_fcn *h, int B);
 /*
  * DenseFCNResNet152.forward, reference models/fcnresnet.py:121-191, for all groups:
@@ -459,7 +459,8 @@ int rcv_i8_quantize_tokens(const void *x0_dev, long long pitch0, int c0, const v
  *               channels rounded up to a multiple of 16 (what lies there has no influence); -128 is allowed
  *   weights     [out_channels][taps][channels rounded up to a multiple of 128], 16-byte aligned, zeros behind `channels`
  *   bias        [out_channels] or NULL; residual [rows, residual_pitch] of out_dtype or NULL (may be `out` itself)
- *   ws          device scratch of rcv_i8_*_workspace_bytes (0 where every call of that size runs without)
+ *   ws          device scratch of rcv_i8_*_workspace_bytes (0 where every call of that size runs without).  More rows may need less, as
+ *               only sums of few tiles are divided; no size needs more than 2^24 bytes
  * rows = 0 does nothing.  RCV_E_TOO_LARGE: channels > 131071 (a sum could overflow), out_channels > 2^20, width > 2^16, more rows than a
  * launch has threads for (2^30 with up to 128 output channels), codes_pitch > 2^22 or a pitch of more than 2^24 elements.
  */

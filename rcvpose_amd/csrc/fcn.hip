@@ -5152,7 +5152,8 @@ I8Scratch i8_scratch(const rcv_fcn *h, const rcv_op &o, int B)
     I8Scratch s;
     s.scales = align_up((size_t)rows * h->groups * align_up((size_t)C, 16), 256);
     s.partial = align_up(s.scales + (size_t)rows * h->groups * 4, 256);
-    s.bytes = align_up(s.partial + i8_product_workspace(rows, C, o.cout, o.ksize * o.ksize, h->groups), 256);
+    // (a bound that grows with the batch: the parts themselves come and go with it, and a workspace of the largest batch serves the others)
+    s.bytes = align_up(s.partial + i8_product_workspace_most(rows, C, o.cout, o.ksize * o.ksize, h->groups), 256);
     return s;
 }
 size_t i8_scratch_bytes(const rcv_fcn *h, int B)

@@ -1132,6 +1132,16 @@ size_t i8_product_workspace(long long rows, int K, int Cout, int taps, int group
     return rows > 0 ? plan_product(rows, K, Cout, taps, groups).bytes : 0;
 }
 
+// plan_product divides a sum while its tiles (of at most 128 x 128) times its parts are at most 256, by channels into eight parts or parts of
+// at least eight steps, by taps into nine.
+size_t i8_product_workspace_most(long long rows, int K, int Cout, int taps, int groups)
+{
+    constexpr long long ALL = 256 * 128 * 128 * 4;
+    if (rows <= 0) return 0;
+    const long long parts = taps == 9 ? 9 : std::max(8, (K + 127) / 128 / 8), row = parts * groups * ((Cout + 3) / 4) * 16;
+    return (size_t)(rows > ALL / row ? ALL : rows * row);
+}
+
 int i8_product(const I8Product &p, void *ws, size_t ws_bytes, hipStream_t st)
 {
     if (p.rows == 0) return RCV_OK;

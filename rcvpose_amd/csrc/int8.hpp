@@ -21,6 +21,8 @@ struct I8Product {
 int i8_quantize(const void *x0, long long pitch0, int c0, const void *x1, long long pitch1, int c1, int dtype, long long rows,
                 int8_t *codes, long long codes_pitch, float *scales, hipStream_t st);
 size_t i8_product_workspace(long long rows, int K, int Cout, int taps, int groups);
+// No less than i8_product_workspace of these or of fewer rows.
+size_t i8_product_workspace_most(long long rows, int K, int Cout, int taps, int groups);
 int i8_product(const I8Product &p, void *ws, size_t ws_bytes, hipStream_t st);
 
 constexpr int I8_KP = 128;  // weight rows are padded with zeros to a multiple of this many codes per tap

@@ -156,3 +156,17 @@ def test_pipeline_runs_the_int8_engine(sds):
         again = pipe.engine.forward(pipe.x)
     torch.cuda.synchronize()
     assert torch.equal(again[1], want[1])
+
+
+@pytest.mark.parametrize("dtype, int8", [("bf16", True), ("fp16", True), ("bf16", r"conv6|block4.*|conv_up1\.0")])
+def test_a_workspace_of_a_larger_batch_serves_a_smaller_one(sds, x, dtype, int8):
+    """Sums are divided where the tiles are few, so a smaller batch may need parts that a larger one does not: the workspace holds them."""
+    eng = FcnEngine(sds[:1], 64, 96, dtype=dtype, int8=int8)
+    sizes = [eng.workspace_bytes(b) for b in range(1, 129)]
+    assert sizes == sorted(sizes)
+    many = x[:1].repeat(17, 1, 1, 1)
+    many.mul_(torch.linspace(0.5, 1.5, 17, device="cuda").view(17, 1, 1, 1))
+    eng.forward(many)
+    got = eng.forward(many[:16])
+    want = FcnEngine(sds[:1], 64, 96, dtype=dtype, int8=int8).forward(many[:16])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

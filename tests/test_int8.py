@@ -200,3 +200,24 @@ def test_main_takes_int8():
     assert main.build_parser().parse_args([]).int8 is False
     opts = main.build_parser().parse_args(["--dtype", "bf16", "--int8", "true"])
     assert opts.int8 is True and opts.dtype == "bf16"
+
+
+def test_workspace_bounds():
+    """The partial sums of a divided product: at most 2^24 bytes, and at most what an engine reserves for a layer whatever the batch (nine
+    parts of a window, for a product eight or one per eight steps of 128 channels).  The sums of one batch may be divided where those
+    of a larger one are not."""
+    lib = _hip.load_library()
+    rng = np.random.default_rng(2)
+    log = lambda lo, hi: int(round(lo * (hi / lo) ** rng.random()))
+    sizes = [(log(1, 1 << 20), log(1, 131071), log(1, 1 << 16)) for _ in range(20000)]
+    sizes += [(rows, k, n) for k, n in ((131071, 1), (131071, 100), (131071, 1000), (20000, 1300), (2048, 1024), (512, 64)) for rows in range(1, 2000)]
+    divided = 0
+    for taps, name in ((1, "rcv_i8_matmul_workspace_bytes"), (9, "rcv_i8_conv3x3_workspace_bytes")):
+        fn = getattr(lib, name)
+        for rows, k, n in sizes:
+            need = fn(rows, k, n)
+            divided += need > 0
+            parts = 9 if taps == 9 else max(8, -(-k // 128) // 8)
+            assert need <= min(1 << 24, parts * rows * -(-n // 4) * 16), (taps, rows, k, n)
+    assert divided > 1000
+    assert lib.rcv_i8_conv3x3_workspace_bytes(2000, 1024, 1024) < lib.rcv_i8_conv3x3_workspace_bytes(500, 1024, 1024)
