@@ -26,20 +26,23 @@ _DTYPES = {torch.float32: _hip.RCV_F32, torch.bfloat16: _hip.RCV_BF16, torch.flo
 
 
 class Int8Weight:
-    """Packed weights of one layer: `codes` int8 [N, taps, K padded to a multiple of 128], `scales` float32 [N].
-    taps is 1 (matmul) or 9 (conv3x3)."""
+    """Packed weights of one layer: `codes` int8 [N, taps, K padded with zeros to a multiple of 128], `scales` float32 [N].
+    taps is 1 (matmul) or 9 (conv3x3).  The padding is looked at once, here: what lies behind a token's last code is anything, and only
+    zeros keep it out of the sums."""
 
-    def __init__(self, codes, scales, channels):
+    def __init__(self, codes, scales, channels, _padded=False):
         if (codes.dtype != torch.int8 or codes.dim() != 3 or codes.shape[0] == 0 or codes.shape[1] not in (1, 9) or not codes.is_contiguous() or
                 not 1 <= channels <= MAX_CHANNELS or codes.shape[2] != (channels + KP - 1) // KP * KP):
             raise ValueError("packed weight codes must be contiguous int8 [N, 1 or 9, channels padded to a multiple of %d]: see pack_codes" % KP)
         if scales.dtype != torch.float32 or tuple(scales.shape) != (codes.shape[0],) or not scales.is_contiguous() or scales.device != codes.device:
             raise ValueError("weight scales must be contiguous float32 [N] on the codes' device")
+        if not _padded and bool(codes[:, :, channels:].any()):
+            raise ValueError("packed weight codes must be zero behind their %d channels: see pack_codes" % channels)
         self.codes, self.scales, self.channels = codes, scales, channels
         self.out_channels, self.taps = int(codes.shape[0]), int(codes.shape[1])
 
     def to(self, device):
-        return Int8Weight(self.codes.to(device), self.scales.to(device), self.channels)
+        return Int8Weight(self.codes.to(device), self.scales.to(device), self.channels, _padded=True)
 
     def dequantize(self):
         """float32 [N, K] or [N, 3, 3, C]: the values the codes stand for."""
@@ -59,7 +62,7 @@ def pack_codes(codes, scales):
     taps = 1 if codes.dim() == 2 else 9
     packed = torch.zeros(n, taps, (k + KP - 1) // KP * KP, dtype=torch.int8, device=codes.device)
     packed[:, :, :k] = codes.reshape(n, taps, k)
-    return Int8Weight(packed, scales.contiguous(), int(k))
+    return Int8Weight(packed, scales.contiguous(), int(k), _padded=True)
 
 
 def quantize_weight(w):

@@ -221,3 +221,17 @@ def test_workspace_bounds():
             assert need <= min(1 << 24, parts * rows * -(-n // 4) * 16), (taps, rows, k, n)
     assert divided > 1000
     assert lib.rcv_i8_conv3x3_workspace_bytes(2000, 1024, 1024) < lib.rcv_i8_conv3x3_workspace_bytes(500, 1024, 1024)
+
+
+@pytest.mark.parametrize("shape", [(8, 40), (5, 3, 3, 130)])
+def test_packed_weight_with_codes_behind_its_channels_is_refused(shape):
+    """They would meet whatever lies behind a token's last code."""
+    good = int8.pack_codes(torch.ones(shape, dtype=torch.int8), torch.ones(shape[0]))
+    k = shape[-1]
+    int8.Int8Weight(good.codes.clone(), good.scales, k)
+    for at in ((0, 0, k), (shape[0] - 1, good.taps - 1, good.codes.shape[2] - 1)):
+        codes = good.codes.clone()
+        codes[at] = -1
+        with pytest.raises(ValueError):
+            int8.Int8Weight(codes, good.scales, k)
+    int8.Int8Weight(torch.ones(4, 1, 128, dtype=torch.int8), torch.ones(4), 128)  # (no padding to look at)
