@@ -56,6 +56,7 @@ def pack_codes(codes, scales):
         raise ValueError("weight codes must be int8 [N, K] or [N, 3, 3, C]")
     if scales.dtype != torch.float32 or tuple(scales.shape) != (codes.shape[0],) or scales.device != codes.device:
         raise ValueError("weight scales must be float32 [N] on the codes' device")
+    scales = scales.detach()
     n, k = codes.shape[0], codes.shape[-1]
     if n == 0 or k == 0 or k > MAX_CHANNELS:
         raise ValueError("an int8 weight needs at least one row and 1 ... %d channels" % MAX_CHANNELS)
@@ -70,6 +71,7 @@ def quantize_weight(w):
     (in float64, on w's device: done once per layer).  A channel of zeros gets scale 0; non-finite weights raise ValueError."""
     if not w.is_floating_point() or w.dim() not in (2, 4):
         raise ValueError("weights must be floating point [N, K] or [N, 3, 3, C]")
+    w = w.detach()  # (a layer's parameter: the scales must not hold its graph)
     flat = w.reshape(w.shape[0], -1).double()
     if flat.numel() and not bool(torch.isfinite(flat).all()):
         raise ValueError("weights are not finite")

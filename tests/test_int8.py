@@ -235,3 +235,12 @@ def test_packed_weight_with_codes_behind_its_channels_is_refused(shape):
         with pytest.raises(ValueError):
             int8.Int8Weight(codes, good.scales, k)
     int8.Int8Weight(torch.ones(4, 1, 128, dtype=torch.int8), torch.ones(4), 128)  # (no padding to look at)
+
+
+def test_weights_of_a_parameter_hold_no_graph():
+    w = torch.nn.Parameter(torch.randn(6, 20))
+    q = int8.quantize_weight(w)
+    assert not q.scales.requires_grad and q.scales.grad_fn is None and not q.dequantize().requires_grad
+    assert torch.equal(q.scales, int8.quantize_weight(w.detach()).scales)
+    p = int8.pack_codes(torch.ones(6, 20, dtype=torch.int8), torch.ones(6, requires_grad=True) * 2)
+    assert not p.scales.requires_grad
