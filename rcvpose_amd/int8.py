@@ -71,11 +71,13 @@ def quantize_weight(w):
     (in float64, on w's device: done once per layer).  A channel of zeros gets scale 0; non-finite weights raise ValueError."""
     if not w.is_floating_point() or w.dim() not in (2, 4):
         raise ValueError("weights must be floating point [N, K] or [N, 3, 3, C]")
+    if w.numel() == 0:
+        raise ValueError("an int8 weight needs at least one row and 1 ... %d channels" % MAX_CHANNELS)
     w = w.detach()  # (a layer's parameter: the scales must not hold its graph)
     flat = w.reshape(w.shape[0], -1).double()
-    if flat.numel() and not bool(torch.isfinite(flat).all()):
+    if not bool(torch.isfinite(flat).all()):
         raise ValueError("weights are not finite")
-    scales = (flat.abs().amax(dim=1) / 127).float() if flat.numel() else torch.zeros(w.shape[0], device=w.device)
+    scales = (flat.abs().amax(dim=1) / 127).float()
     scales = torch.where(scales < 2.0 ** -126, torch.zeros_like(scales), scales)
     if not bool(torch.isfinite(scales).all()):
         raise ValueError("weights are beyond float32's range")

@@ -244,3 +244,9 @@ def test_weights_of_a_parameter_hold_no_graph():
     assert torch.equal(q.scales, int8.quantize_weight(w.detach()).scales)
     p = int8.pack_codes(torch.ones(6, 20, dtype=torch.int8), torch.ones(6, requires_grad=True) * 2)
     assert not p.scales.requires_grad
+
+
+@pytest.mark.parametrize("shape", [(0, 16), (4, 0), (0, 3, 3, 16), (4, 3, 3, 0)])
+def test_weights_without_a_row_or_a_channel_are_refused(shape):
+    with pytest.raises(ValueError):
+        int8.quantize_weight(torch.ones(shape))
