@@ -86,9 +86,9 @@ def quantize_weight(w):
     return pack_codes(codes.clamp_(-127, 127).to(torch.int8).view(w.shape), scales)
 
 
-def _rows(t):
+def _rows(t, border=1):
     """A channels-last tensor as (tensor, number of rows, row pitch in elements); anything whose leading dimensions do not walk rows at
-    one pitch is copied."""
+    one pitch is copied, to rows that start a multiple of `border` elements apart (rows that overlap: one behind the other)."""
     c = t.shape[-1]
     if t.is_contiguous():
         return t, t.numel() // c if c else 0, c
@@ -105,8 +105,11 @@ def _rows(t):
         pitch = c if pitch is None else pitch
         if uniform and pitch >= c:
             return t, rows, pitch
-    t = t.contiguous()
-    return t, t.numel() // c, c
+        if uniform and pitch:
+            border = 1
+    pitch = (c + border - 1) // border * border
+    copy = t.contiguous() if pitch == c else torch.empty(*t.shape[:-1], pitch, dtype=t.dtype, device=t.device)[..., :c].copy_(t)
+    return copy, t.numel() // c, pitch
 
 
 def _elsewhere(t):
@@ -199,7 +202,7 @@ def _product(codes, scales, weight, bias, residual, relu, dtype, height, width):
             _elsewhere(residual)
         residual, _, res_pitch = _rows(residual)
         res_ptr = residual.data_ptr()
-    codes, rows, pitch = _rows(codes)
+    codes, rows, pitch = _rows(codes, 16)
     if rows == 0:
         return out
     ptr, need = codes.data_ptr(), (k + 15) // 16 * 16

@@ -533,3 +533,18 @@ def test_tall_images(h, n):
         v, mag = ref_product(a[part].cpu().numpy(), sa[part].cpu().numpy(), w.cpu().numpy().reshape(n, 9, c), sw.cpu().numpy(), f64(bias), None, False,
                              (1, m + 1, 1))
         check_product(got[part][first:last], v[first:last], mag[first:last], dtype, 9)
+
+
+@pytest.mark.parametrize("c", [64, 40, 33, 1])
+def test_views_of_quantised_images(c):
+    """Crops, every second row, and a transposition of quantise_tokens' codes walk memory at no single pitch: they are copied, whatever the
+    number of channels."""
+    torch.manual_seed(c)
+    codes, scales = int8.quantize_tokens(torch.randn(2, 9, 10, c, device="cuda"))
+    wc, wm = int8.quantize_weight(torch.randn(24, 3, 3, c, device="cuda")), int8.quantize_weight(torch.randn(24, c, device="cuda"))
+    for view in (lambda t: t[:, 1:-1, 1:-1], lambda t: t[:, ::2], lambda t: t.transpose(1, 2), lambda t: t[:, :, ::3], lambda t: t[:1, 2:3], lambda t: t[:, 3:4, 5:6]):
+        q, s = view(codes), view(scales)
+        whole = torch.zeros(*q.shape[:-1], (c + 15) // 16 * 16, dtype=torch.int8, device="cuda")
+        whole[..., :c] = q
+        for call, w in ((int8.conv3x3, wc), (int8.matmul, wm)):
+            assert torch.equal(call(q, s, w, dtype=torch.float32), call(whole[..., :c], s.contiguous(), w, dtype=torch.float32))
