@@ -86,9 +86,9 @@ def quantize_weight(w):
     return pack_codes(codes.clamp_(-127, 127).to(torch.int8).view(w.shape), scales)
 
 
-def _rows(t, border=1):
+def _rows(t, border=1, farthest=1 << 24):
     """A channels-last tensor as (tensor, number of rows, row pitch in elements); anything whose leading dimensions do not walk rows at
-    one pitch is copied, to rows that start a multiple of `border` elements apart (rows that overlap: one behind the other)."""
+    one pitch of up to `farthest` is copied, to rows that start a multiple of `border` elements apart (rows that overlap: one behind the other)."""
     c = t.shape[-1]
     if t.is_contiguous():
         return t, t.numel() // c if c else 0, c
@@ -103,9 +103,9 @@ def _rows(t, border=1):
                 uniform = False
             rows *= size
         pitch = c if pitch is None else pitch
-        if uniform and pitch >= c:
+        if uniform and c <= pitch <= farthest:
             return t, rows, pitch
-        if uniform and pitch:
+        if uniform and 0 < pitch < c:
             border = 1
     pitch = (c + border - 1) // border * border
     copy = t.contiguous() if pitch == c else torch.empty(*t.shape[:-1], pitch, dtype=t.dtype, device=t.device)[..., :c].copy_(t)
@@ -202,7 +202,7 @@ def _product(codes, scales, weight, bias, residual, relu, dtype, height, width):
             _elsewhere(residual)
         residual, _, res_pitch = _rows(residual)
         res_ptr = residual.data_ptr()
-    codes, rows, pitch = _rows(codes, 16)
+    codes, rows, pitch = _rows(codes, 16, 1 << 22)
     if rows == 0:
         return out
     ptr, need = codes.data_ptr(), (k + 15) // 16 * 16

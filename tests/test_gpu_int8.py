@@ -548,3 +548,22 @@ def test_views_of_quantised_images(c):
         whole[..., :c] = q
         for call, w in ((int8.conv3x3, wc), (int8.matmul, wm)):
             assert torch.equal(call(q, s, w, dtype=torch.float32), call(whole[..., :c], s.contiguous(), w, dtype=torch.float32))
+
+
+@pytest.mark.parametrize("c", [64, 40])
+def test_rows_farther_apart_than_the_kernels_take(c):
+    """A few channels of very wide matrices: x, codes and the residual are copied where their rows lie beyond the kernels' pitches."""
+    torch.manual_seed(c)
+    weight = int8.quantize_weight(torch.randn(24, c, device="cuda"))
+    x = torch.zeros(3, (1 << 24) + 16, dtype=torch.bfloat16, device="cuda")[:, 8:8 + c]
+    x.normal_()
+    codes, scales = int8.quantize_tokens(x)
+    want = int8.quantize_tokens(x.contiguous())
+    assert torch.equal(codes, want[0]) and torch.equal(scales, want[1])
+    far = torch.full((3, (1 << 22) + 16), 99, dtype=torch.int8, device="cuda")[:, 16:16 + c]
+    far.copy_(codes)
+    res = torch.zeros(3, (1 << 24) + 16, dtype=torch.float16, device="cuda")[:, 1:25]
+    res.normal_()
+    y = int8.matmul(codes, scales, weight, residual=res.contiguous(), dtype=torch.float16)
+    assert torch.equal(int8.matmul(far, scales, weight, residual=res, dtype=torch.float16), y)
+    assert torch.equal(int8.quantize_tokens(x, x)[1], scales)
