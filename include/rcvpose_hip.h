@@ -461,6 +461,7 @@ int rcv_i8_quantize_tokens(const void *x0_dev, long long pitch0, int c0, const v
  *   bias        [out_channels] or NULL; residual [rows, residual_pitch] of out_dtype or NULL (may be `out` itself)
  *   ws          device scratch of rcv_i8_*_workspace_bytes (0 where every call of that size runs without).  More rows may need less, as
  *               only sums of few tiles are divided; no size needs more than 2^24 bytes
+ * Scales, bias, residual and out are aligned to their elements, ws to 16 bytes.
  * rows = 0 does nothing.  RCV_E_TOO_LARGE: channels > 131071 (a sum could overflow), out_channels > 2^20, width > 2^16, more rows than a
  * launch has threads for (2^30 with up to 128 output channels), codes_pitch > 2^22 or a pitch of more than 2^24 elements.
  */

@@ -1171,6 +1171,7 @@ int check_args(const rcv_i8_args *a, int taps, I8Product &p)
     if (!a->codes_dev || !a->code_scales_dev || !a->weights_dev || !a->weight_scales_dev || !a->out_dev) return RCV_E_INVALID;
     if ((uintptr_t)a->codes_dev % 16 || (uintptr_t)a->weights_dev % 16 || a->codes_pitch % 16 || a->codes_pitch < a->channels)
         return RCV_E_INVALID;
+    if ((uintptr_t)a->code_scales_dev % 4 || (uintptr_t)a->weight_scales_dev % 4 || (uintptr_t)a->bias_dev % 4) return RCV_E_INVALID;
     if (a->codes_pitch > (1 << 22) || a->out_pitch > (1 << 24) || (a->residual_dev && a->residual_pitch > (1 << 24))) return RCV_E_TOO_LARGE;
     const int size = a->out_dtype == RCV_F32 ? 4 : 2;
     if ((uintptr_t)a->out_dev % size || a->out_pitch < a->out_channels) return RCV_E_INVALID;
@@ -1199,6 +1200,7 @@ int rcv_i8_quantize_tokens(const void *x0_dev, long long pitch0, int c0, const v
     if (!float_type(dtype)) return RCV_E_UNSUPPORTED;
     if (c0 > I8_MAX_K || c1 > I8_MAX_K - c0 || rows > I8_MAX_ROWS) return RCV_E_TOO_LARGE;
     const int size = dtype == RCV_F32 ? 4 : 2;
+    if ((uintptr_t)scales_dev % 4) return RCV_E_INVALID;
     if ((uintptr_t)x0_dev % size || (uintptr_t)x1_dev % size || pitch0 < c0 || (c1 && pitch1 < c1) || codes_pitch < c0 + c1) return RCV_E_INVALID;
     if (pitch0 > (1 << 24) || (c1 && pitch1 > (1 << 24)) || codes_pitch > (1 << 24) || rows > 0x7fffffff) return RCV_E_TOO_LARGE;
     return i8_quantize(x0_dev, pitch0, c0, x1_dev, pitch1, c1, dtype, rows, codes_dev, codes_pitch, scales_dev, (hipStream_t)stream);

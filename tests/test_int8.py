@@ -250,3 +250,16 @@ def test_weights_of_a_parameter_hold_no_graph():
 def test_weights_without_a_row_or_a_channel_are_refused(shape):
     with pytest.raises(ValueError):
         int8.quantize_weight(torch.ones(shape))
+
+
+@pytest.mark.parametrize("name", ["rcv_i8_matmul", "rcv_i8_conv3x3"])
+@pytest.mark.parametrize("field", ["code_scales", "weight_scales", "bias"])
+def test_product_refuses_numbers_off_their_alignment(name, field):
+    for off in (1, 2, 3):
+        assert _call(name, _args(rows=0, **{field: FAKE + off})) == _hip.RCV_E_INVALID
+    assert _call(name, _args(rows=0, **{field: FAKE + 4})) == _hip.RCV_OK
+
+
+def test_quantize_refuses_scales_off_their_alignment():
+    for off, status in ((2, _hip.RCV_E_INVALID), (4, _hip.RCV_OK)):
+        assert _hip.load_library().rcv_i8_quantize_tokens(FAKE, 64, 64, None, 0, 0, _hip.RCV_F32, 0, FAKE, 64, FAKE + off, None) == status
