@@ -403,6 +403,9 @@ def pack_weights(state_dicts, builder, ops, dtype, q6=False, int8=False):
     sds = [{(k[7:] if k.startswith("module.") else k): v for k, v in sd.items()} for sd in state_dicts]
     tdt = {_hip.RCV_F32: torch.float32, _hip.RCV_BF16: torch.bfloat16, _hip.RCV_F16: torch.float16,
            _hip.RCV_F16X3: torch.float16}[dtype]
+    pattern8 = (INT8_DEFAULT if int8 is True else int8) if int8 and dtype in (_hip.RCV_BF16, _hip.RCV_F16) else None
+    if pattern8 and not any(spec is not None and int8_wanted(spec, op, pattern8) for op, spec in zip(ops, builder.wspecs)):
+        raise ValueError("int8 pattern %r names no stride-1 1x1 or 3x3 convolution of this network" % pattern8)
     wparts, bparts, woff, boff = [], [], 0, 0
     for idx, (op, spec) in enumerate(zip(ops, builder.wspecs)):
         op["wq_off"] = 0
@@ -412,7 +415,7 @@ def pack_weights(state_dicts, builder, ops, dtype, q6=False, int8=False):
         ws, bs, wq, bq = [], [], [], []
         want_q6 = bool(q6) and dtype == _hip.RCV_F16X3 and q6_wanted(spec, op, Q6_DEFAULT if q6 is True else q6)
         want_tailc = dtype == _hip.RCV_F16X3 and tail_composed_wanted(builder, idx)
-        want_int8 = bool(int8) and dtype in (_hip.RCV_BF16, _hip.RCV_F16) and int8_wanted(spec, op, INT8_DEFAULT if int8 is True else int8)
+        want_int8 = bool(pattern8) and int8_wanted(spec, op, pattern8)
         for sd in sds:
             w, b = fold_conv_bn(sd, spec, op["cout"])
             wmax = float(w.abs().max()) if w.numel() else 0.0
@@ -478,7 +481,7 @@ class FcnEngine:
     the split product as one block-scaled fp6 matrix instruction (engine option 11, q6_wanted): -18 % on those launches, -3 % on
     the forward, for 2-3x the map error (worst network of the bench 3.4e-5 -> 7.8e-5 of the 1e-4 tolerance: r05 measurement).
     int8 (bf16 / fp16; default off): True or a regex over convolution names -- those stride-1 convolutions run on 8-bit integers with one
-    scale per pixel and output channel (engine option 16, int8_wanted).  Their maps may differ between batch sizes by the rounding of a
+    scale per pixel and output channel (engine option 16, int8_wanted); a regex that names none raises ValueError.  Their maps may differ between batch sizes by the rounding of a
     float32 sum (the nine taps of a window are added in an order that depends on the batch).
     """
 

@@ -263,3 +263,16 @@ def test_product_refuses_numbers_off_their_alignment(name, field):
 def test_quantize_refuses_scales_off_their_alignment():
     for off, status in ((2, _hip.RCV_E_INVALID), (4, _hip.RCV_OK)):
         assert _hip.load_library().rcv_i8_quantize_tokens(FAKE, 64, 64, None, 0, 0, _hip.RCV_F32, 0, FAKE, 64, FAKE + off, None) == status
+
+
+@pytest.mark.parametrize("arch", ["dense", "res"])
+def test_a_pattern_that_names_no_convolution_is_refused(arch):
+    """A misspelt layer would leave an engine without an int8 layer; so would names whose convolutions the integer kernels do not run."""
+    from rcvpose_amd import fcn_engine
+
+    b = (fcn_engine.build_program if arch == "dense" else fcn_engine.build_program_res)(64, 96)
+    ops = fcn_engine.assign_slots(b)[0]
+    for pattern in ("typo", "conv_up4", r"conv1", r"block2up\.conv2"):
+        for dtype in (_hip.RCV_BF16, _hip.RCV_F16):
+            with pytest.raises(ValueError, match="int8"):
+                fcn_engine.pack_weights([], b, ops, dtype, int8=pattern)
