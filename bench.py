@@ -63,7 +63,10 @@ def parse(argv=None):
                          "all_reduce of the N-rank path in a one-rank group (exercises that path on a one-GPU box)")
     ap.add_argument("--selftest-launcher", action="store_true",
                     help="CPU only: exercise the launcher / rendezvous / gather with gloo ranks and no GPU work (tests)")
-    return ap.parse_args(argv)
+    args = ap.parse_args(argv)
+    if args.int8 and args.dtype not in ("bf16", "fp16"):
+        ap.error("--int8 needs --dtype bf16 or fp16")
+    return args
 
 
 # ---------------------------------------------------------------------------------------------------------
@@ -390,7 +393,7 @@ def main(argv=None):
     sds = [{k: torch.from_numpy(v) for k, v in synthetic_weights.make_state_dict_numpy(shapes, seed=s).items()}
            for s in range(G)]
     pipe = FramePipeline(sds, H, W, dtype=args.dtype, frames_per_step=B, overlap=args.overlap, q6=args.q6 and args.dtype == "f16x3",
-                         int8=args.int8 and args.dtype in ("bf16", "fp16"))
+                         int8=args.int8)
 
     # frames are sharded over ranks: global frame f -> rank f % world; local frame i of rank r is the
     # synthetic frame r + world * i.  A pool of distinct frames per rank is cycled, resident in HBM before the timed region.
@@ -605,7 +608,7 @@ def main(argv=None):
                                       "the LDS shell rasteriser (k_vote) is its fallback and is timed in extras.rasteriser_engine_frames_per_s",
                        "frames_per_step_per_gpu": B, "distinct_frames_cycled": pool,
                        "weights": "random (seeded He), ideal maps injected after the forward",
-                       "overlap": bool(args.overlap), "q6_cross_terms": bool(args.q6 and args.dtype == "f16x3"), "int8_decoder": bool(args.int8 and args.dtype in ("bf16", "fp16")), "parallelism": "frames sharded f%%%d, 1 RCCL all_gather/step" % world},
+                       "overlap": bool(args.overlap), "q6_cross_terms": bool(args.q6 and args.dtype == "f16x3"), "int8_decoder": bool(args.int8), "parallelism": "frames sharded f%%%d, 1 RCCL all_gather/step" % world},
             "roofline": {"bound": "mfma", "achieved": achieved, "peak": peak, "unit": "TFLOP/s", "frac": achieved / peak,
                          "traffic": traffic, "traffic_unit": "HBM bytes per step (all conv launches)", "traffic_source": traffic_src,
                          "algorithmic_flop_per_step": conv_flop_step,

@@ -40,6 +40,8 @@ def build_parser():
 
 def main(argv=None):
     opts = build_parser().parse_args(argv)
+    if opts.int8 and opts.dtype not in ('bf16', 'fp16'):
+        raise SystemExit("--int8 needs --dtype bf16 or fp16")
     opts.cfg = get_config()[1]
     if opts.mode != 'test':
         raise SystemExit("rcvpose_amd implements --mode=test (the inference hot path); use the reference for training")

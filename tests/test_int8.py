@@ -276,3 +276,18 @@ def test_a_pattern_that_names_no_convolution_is_refused(arch):
         for dtype in (_hip.RCV_BF16, _hip.RCV_F16):
             with pytest.raises(ValueError, match="int8"):
                 fcn_engine.pack_weights([], b, ops, dtype, int8=pattern)
+
+
+@pytest.mark.parametrize("dtype", [None, "f16x3", "fp32"])
+def test_commands_refuse_int8_with_other_types(dtype, capsys):
+    """The bench dropped the flag silently, main.py went as far as building the engine."""
+    import bench
+    from rcvpose_amd import main
+
+    extra = [] if dtype is None else ["--dtype", dtype]
+    with pytest.raises(SystemExit):
+        bench.parse(["--int8"] + extra)
+    with pytest.raises(SystemExit, match="int8"):
+        main.main(["--int8", "true", "--mode", "test"] + extra)
+    capsys.readouterr()
+    assert bench.parse(["--int8", "--dtype", "fp16"]).int8 is True and bench.parse([]).int8 is False
