@@ -25,6 +25,8 @@ class FramePipeline:
         input size (BN folding, weight packing and upload take seconds: a caller that sizes its batch first builds the engine once)."""
         import torch
 
+        if fcn is not None and int8:
+            raise ValueError("int8 is chosen where the engine is built: FcnEngine(int8=...), handed in as fcn")
         assert len(state_dicts) >= 1
         self.torch = torch
         self.lib = _hip.lib()

@@ -291,3 +291,10 @@ def test_commands_refuse_int8_with_other_types(dtype, capsys):
         main.main(["--int8", "true", "--mode", "test"] + extra)
     capsys.readouterr()
     assert bench.parse(["--int8", "--dtype", "fp16"]).int8 is True and bench.parse([]).int8 is False
+
+
+def test_pipeline_refuses_int8_for_an_engine_that_is_built():
+    from rcvpose_amd.pipeline import FramePipeline
+
+    with pytest.raises(ValueError, match="int8"):
+        FramePipeline([{}], 64, 96, dtype="bf16", fcn=object(), int8=True)
