@@ -8,7 +8,8 @@
 A token is one row of a channels-last tensor; its value is codes * scale.  FcnEngine(int8=...) runs chosen convolutions of the FCN on
 these kernels.  Inference only: no gradient flows through; there is no CPU fallback.  Results do not depend on the run: integer sums are exact and float sums
 have an order that the sizes alone decide (matmul gives a token the same bits in any batch; conv3x3's nine taps may be added in another
-order in a batch of another size).  The reference has no counterpart (its forward is fp32, models/fcnresnet.py:121-191).
+order in a batch of another size, so that the last bits of the float32 sum differ and its rounding to 16 bits may fall to the other side).
+The reference has no counterpart (its forward is fp32, models/fcnresnet.py:121-191).
 """
 import ctypes
 import struct

@@ -32,7 +32,8 @@ def build_parser():
                    help="bf16 / fp16 only: the decoder's wide 3x3 convolutions on 8-bit integers (one scale per pixel and output channel)")
     p.add_argument('--frames_per_step', type=int, default=53,
                    help="frames of a class that travel through the device pipeline together (LINEMOD loop with checkpoints; default: "
-                        "bench.py's batch); results do not depend on it (with --int8: but for the order in which float32 adds nine numbers)")
+                        "bench.py's batch); results do not depend on it (with --int8 they may: float32 sums are added in an order that the batch decides, "
+                        "and maps can differ by some 1e-2 of their range at a few pixels)")
     p.add_argument('--eval_threads', type=int, default=default_eval_threads(),
                    help="host threads (one HIP stream each) for the per-frame Horn / ADD(-S) / ICP evaluation of a batch")
     return p

@@ -170,3 +170,34 @@ def test_a_workspace_of_a_larger_batch_serves_a_smaller_one(sds, x, dtype, int8)
     got = eng.forward(many[:16])
     want = FcnEngine(sds[:1], 64, 96, dtype=dtype, int8=int8).forward(many[:16])
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_an_image_alone_and_among_others(sds, x, dtype):
+    """A batch of another size may divide a window's sum otherwise.  The first int8 layer has the same source in both, bit for bit; its two
+    results are within 31 roundings of float32 (nine taps, up to sixteen partial sums, scale, bias, residual) of one real number each,
+    and are then rounded by at most half a step of the stored type.  What the layers behind make of a moved step is printed."""
+    engines = [FcnEngine(sds[:1], 64, 96, dtype=dtype, reuse_slots=False, int8=True) for _ in range(2)]
+    batches = (1, 17)
+    many = x[:1].repeat(17, 1, 1, 1)
+    many[1:] *= 0.7
+    maps = [eng.forward(many[:b])[1][0, 0, 0] for eng, b in zip(engines, batches)]
+    builder = fcn_engine.build_program(64, 96)
+    first = next(i for i, op in enumerate(engines[0].ops) if op["wq_off"])
+    op, spec = engines[0].ops[first], builder.wspecs[first]
+    assert spec["conv"] == "conv6" and op["src1"] < 0 and op["res"] < 0
+    src = [eng.debug_slot(b, 0, op["src0"], (op["hin"], op["win"], op["c0"]))[0] for eng, b in zip(engines, batches)]
+    out = [eng.debug_slot(b, 0, op["dst"], (op["hout"], op["wout"], op["cout"]))[0].double() for eng, b in zip(engines, batches)]
+    assert torch.equal(src[0], src[1])
+    w, bias = fcn_engine.fold_conv_bn(sds[0], spec, op["cout"])
+    weight = int8.quantize_weight(w).to("cuda")
+    codes, scales = int8.quantize_tokens(src[0][None].to(TORCH[dtype]))
+    size = int8.conv3x3(codes.abs(), scales, int8.pack_codes(weight.codes[:, :, :weight.channels].abs().reshape(w.shape), weight.scales),
+                        bias=bias.float().abs().cuda(), dtype=torch.float32)[0].double()
+    eps = torch.finfo(TORCH[dtype]).eps
+    diff = (out[0] - out[1]).abs()
+    assert bool((diff <= 62 * 2.0 ** -24 * size * (1 + eps) + eps * out[1].abs() * (1 + eps) + 2.0 ** -24).all()), float(diff.max())
+    assert float(out[1].abs().max()) > 0
+    print("%s: image alone and among 17: radial maps differ by %.2e of their range" % (dtype, float((maps[0] - maps[1]).abs().max() / maps[1].abs().max())))
+    again = [eng.forward(many[:b])[1][0, 0, 0] for eng, b in zip(engines, batches)]
+    assert torch.equal(again[0], maps[0]) and torch.equal(again[1], maps[1])  # (in one batch size: the same bits)
