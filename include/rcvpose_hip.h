@@ -451,10 +451,12 @@ int rcv_i8_quantize_tokens(const void *x0_dev, long long pitch0, int c0, const v
  * out[m, n] = act( sw[n] * sum_tap sa[m(tap)] * (sum_k codes[m(tap), k] * weights[n, tap, k]) + bias[n] + residual[m, n] )
  *
  * rcv_i8_matmul: one tap, m(tap) = m.  rcv_i8_conv3x3: the nine taps of a 3x3 window with zero padding and stride 1 over images of
- * height x width tokens (rows = images * height * width, row-major).  Sums within a tap are exact 32-bit integers, taps are added
- * in float32 in an order that the sizes alone decide, the result is rounded once to out_dtype: two calls of one size give the same bits.
- * (rcv_i8_matmul gives a row the same bits whatever the other sizes; a window among more or fewer images may differ in its float32
- * sum's last bits.)  ReLU keeps a NaN.
+ * height x width tokens (rows = images * height * width, row-major).  Sums of codes are exact 32-bit integers.  What follows is float32,
+ * each step rounded: the sum's conversion (whole numbers above 2^24), its token scale, the weight scale and the bias in one step, the
+ * residual; the result is then rounded to out_dtype.  rcv_i8_conv3x3 converts and scales the sum of a tap, or of a run of a tap's channels,
+ * and adds these in float32 in an order that the sizes alone decide: two calls of one size give the same bits, a window among more or
+ * fewer images may differ in its float32 sum's last bits, and no result is off by more than 31 roundings of the sum of the magnitudes that
+ * are added.  (rcv_i8_matmul: 4, and a row has the same bits whatever the other sizes.)  ReLU keeps a NaN.
  *   codes       rows codes_pitch bytes apart; 16-byte aligned, codes_pitch a multiple of 16, and the last row readable up to
  *               channels rounded up to a multiple of 16 (what lies there has no influence); -128 is allowed
  *   weights     [out_channels][taps][channels rounded up to a multiple of 128], 16-byte aligned, zeros behind `channels`

@@ -5,7 +5,9 @@
 //   product   out[m, n] = act( sw[n] * sum_tap sa[m(tap)] * (sum_k a[m(tap), k] w[n, tap, k]) + bias[n] + residual[m, n] )
 //             taps = 1: rows x channels; taps = 9: a 3x3 window with zero padding over tokens that form H x W images.  The sums
 //             within a tap are 32-bit integers and exact (|code| <= 128: K <= 131071 cannot overflow); the taps, whose
-//             tokens have scales of their own, are added in float32 in a fixed order.
+//             tokens have scales of their own, are added in float32 in an order that the sizes fix (k_i8_direct: runs of a tap's channels).
+//             Float32, as nothing narrower holds the sums: it rounds the conversion, the token scale, each addition, the weight scale
+//             with the bias and the residual; then the output's type rounds.
 #include <math.h>
 
 #include <algorithm>

@@ -229,7 +229,8 @@ def matmul(codes, scales, weight, bias=None, residual=None, relu=False, dtype=to
     """act( (codes @ weight.T) * scales * weight scales + bias + residual ) -> [..., N] of `dtype`.
 
     codes int8 [..., K] and scales float32 [...] as quantize_tokens gives them, weight an Int8Weight of [N, K], bias float32 [N],
-    residual [..., N] of `dtype`.  The integer sums are exact; the result is rounded once, to `dtype`.  relu keeps a NaN."""
+    residual [..., N] of `dtype`.  The integer sums are exact; float32 rounds their conversion, the product with the token's scale, the weight
+    scale with the bias, and the residual, and the result is rounded to `dtype`.  relu keeps a NaN."""
     if weight.taps != 1:
         raise ValueError("matmul takes a weight packed from [N, K]; a 3x3 weight belongs to conv3x3")
     return _product(codes, scales, weight, bias, residual, relu, dtype, 0, 0)
@@ -238,7 +239,8 @@ def matmul(codes, scales, weight, bias=None, residual=None, relu=False, dtype=to
 def conv3x3(codes, scales, weight, bias=None, residual=None, relu=False, dtype=torch.bfloat16):
     """3x3 convolution with zero padding and stride 1 over tokens that form images: codes int8 [B, H, W, C], scales float32
     [B, H, W], weight an Int8Weight of [N, 3, 3, C] -> [B, H, W, N] of `dtype`.  Every input pixel enters under its own scale: integer
-    sums over the channels of one tap are exact, the nine taps are added in float32.  bias, residual, relu as in matmul."""
+    sums over the channels of one tap, or over runs of them where a sum is divided, are exact, then converted and scaled; these are added
+    in float32.  bias, residual, relu as in matmul."""
     if weight.taps != 9:
         raise ValueError("conv3x3 takes a weight packed from [N, 3, 3, C]")
     if codes.dim() != 4:
