@@ -1081,14 +1081,20 @@ template <typename T, int TAPS, int TT, int CT, int D> int launch_direct(const I
     return partial ? launch_finish<T, TAPS>(p, pl, partial, st) : RCV_OK;
 }
 
-// The shortest sum for which 256 x 256 tiles pay.  256 / 128, us: 16384 rows -> 4096 channels of bfloat16, 512 69 / 71, 768 81 / 86, 1024 91 / 99, 2048
-// 135 / 153, 8192 400 / 483.  They finish from registers, with less to hide it behind: rows that start anywhere (4001 channels: 1024
-// 110 / 100, 1536 133 / 133, 2048 153 / 156) and residuals in pieces of lines (float32: 1024 196 / 153, 2048 239 / 206, 4096 326 / 331; bfloat16,
-// 4008 channels: 1024 126 / 115, 2048 168 / 170) need more.
+// The shortest sum for which 256 x 256 tiles pay.  256 / 128, us, 16384 rows -> 4096 channels: bfloat16, 512 69 / 71, 768 81 / 86, 1024 91 / 99,
+// 2048 135 / 153, 8192 400 / 483; with a residual 768 113 / 121, 2560 192 / 203; float32 768 108 / 100, 1536 144 / 139, 2560 194 / 194, 4096
+// 261 / 278 (in one round, 4096 rows: 768 32 / 32, 2560 51 / 56).  They finish from registers, with less to hide it behind, and some ends
+// need a longer sum to pay for them, each about as much again:
+// - 16-bit rows that start anywhere.  4001 channels: 1536 143 / 130, 2048 163 / 154, 2560 188 / 185, 3328 219 / 226; 4096 rows: 2048 47 / 46,
+//   2560 53 / 54.
+// - residuals in pieces of lines.  bfloat16, 4008 channels: 2048 183 / 175, 2560 207 / 204, 3328 236 / 243.  float32 crosses by the rounds
+//   that are behind each other: 4 (16384 rows) 2048 246 / 216, 2560 275 / 255, 3328 302 / 302, 4096 337 / 339; 2 (8192 rows) 2048 125 / 126,
+//   2560 139 / 142; 1 (4096 rows) 1024 44 / 47, 2560 64 / 69; 4001 channels in 4 rounds 2048 246 / 228, 2560 271 / 268, 3328 302 / 309.
+// - both: 4001 channels of bfloat16 3328 266 / 247, 4096 294 / 291, 4608 318 / 319; 4096 rows 4096 78 / 77, 4608 84 / 84.
 template <typename T> int wide_from(const I8Product &p)
 {
     const long long pitch = p.out_pitch * (long long)sizeof(T);
-    return 768 + (sizeof(T) == 2 && pitch % 16 ? 1024 : 0) + (p.residual && (sizeof(T) == 4 || pitch % 128) ? 1792 : 0);
+    return 768 + (sizeof(T) == 2 && pitch % 16 ? 1792 : 0) + (p.residual && (sizeof(T) == 4 || pitch % 128) ? 1792 : 0);
 }
 
 template <typename T, int TAPS> int launch_taps(const I8Product &p, const Plan &pl, void *ws, hipStream_t st)

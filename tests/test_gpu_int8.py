@@ -567,3 +567,10 @@ def test_rows_farther_apart_than_the_kernels_take(c):
     y = int8.matmul(codes, scales, weight, residual=res.contiguous(), dtype=torch.float16)
     assert torch.equal(int8.matmul(far, scales, weight, residual=res, dtype=torch.float16), y)
     assert torch.equal(int8.quantize_tokens(x, x)[1], scales)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("k", [2300, 2700, 4400])
+def test_matmul_of_many_rows_with_a_residual(k, dtype):
+    """Both sides of the sums from which the widest tiles take odd rows and residuals."""
+    test_matmul(12301, k, 1025, dtype)
