@@ -29,7 +29,8 @@ def build_parser():
                    help="engine arithmetic: f16x3 (default; fp16 hi/lo pairs, 3 MFMAs per product) and fp32 reproduce the reference's "
                         "fp32 forward to 1e-4; bf16 / fp16 are throughput modes outside that tolerance")
     p.add_argument('--int8', type=str2bool, default=False,
-                   help="bf16 / fp16 only: the decoder's wide 3x3 convolutions on 8-bit integers (one scale per pixel and output channel)")
+                   help="bf16 / fp16 only: the decoder's wide 3x3 convolutions on 8-bit integers (one scale per pixel and output channel): some per "
+                        "cent faster, keypoints a few voxels less exact")
     p.add_argument('--frames_per_step', type=int, default=53,
                    help="frames of a class that travel through the device pipeline together (LINEMOD loop with checkpoints; default: "
                         "bench.py's batch); results do not depend on it (with --int8 they may: float32 sums are added in an order that the batch decides, "

@@ -201,3 +201,26 @@ def test_an_image_alone_and_among_others(sds, x, dtype):
     print("%s: image alone and among 17: radial maps differ by %.2e of their range" % (dtype, float((maps[0] - maps[1]).abs().max() / maps[1].abs().max())))
     again = [eng.forward(many[:b])[1][0, 0, 0] for eng, b in zip(engines, batches)]
     assert torch.equal(again[0], maps[0]) and torch.equal(again[1], maps[1])  # (in one batch size: the same bits)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_keypoints_under_the_int8_engines_error(golden_dir, oracle, monkeypatch, dtype):
+    """What the int8 layers' error does to the keypoints, measured as for the other types (test_gpu_pipeline: the error field of a random network,
+    transferred onto ideal maps, against the fp32 engine's keypoints): the figures are printed.  What is asserted is exact: the
+    device votes on the perturbed maps like the oracle, and the int8 layers' error is no smaller than the one of 16 bits they add to."""
+    import numpy as np
+
+    import test_gpu_pipeline as yard
+    from rcvpose_amd import pipeline
+
+    plain = yard._keypoints_under_engine_error(golden_dir, dtype)
+    whole = pipeline.FramePipeline
+    monkeypatch.setattr(pipeline, "FramePipeline", lambda *a, **kw: whole(*a, int8=kw["dtype"] != "fp32", **kw))
+    dev, rel, step, (ps, pr), fr, rmax, kp = yard._keypoints_under_engine_error(golden_dir, dtype)
+    for name, (d, r, s) in ((dtype, plain[:3]), (dtype + " with int8 layers", (dev, rel, step))):
+        print("%s: keypoints move by %.2f voxels at most, %.3f on average, %d of %d by more than one; radial maps %s of their range (radius: max %.2f, "
+              "rms %.2f voxels)" % (name, d.max(), d.mean(), int((d > 1).sum()), d.size, ["%.1e" % e for e, _ in r], s[0], s[1]))
+    assert step[1] > plain[2][1]
+    for b, k in ((0, 0), (3, 1), (7, 2)):
+        xyz, rl = oracle.seam(ps[k, b, 0], pr[k, b, 0], fr[b]["depth"], rmax[k])
+        assert np.array_equal(kp[b, k], oracle.accumulator_3d(xyz, rl, sparse=True)[0])
