@@ -224,3 +224,45 @@ def test_keypoints_under_the_int8_engines_error(golden_dir, oracle, monkeypatch,
     for b, k in ((0, 0), (3, 1), (7, 2)):
         xyz, rl = oracle.seam(ps[k, b, 0], pr[k, b, 0], fr[b]["depth"], rmax[k])
         assert np.array_equal(kp[b, k], oracle.accumulator_3d(xyz, rl, sparse=True)[0])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_res_network(golden_dir, x, dtype):
+    """ResFCNResNet152: two of its decoder's windows by default, and a lateral 1x1 convolution with the upsampled tensor as its residual.  Every op
+    against the public operators (the bound of test_every_int8_op_equals_the_public_operators), the model class against the engine."""
+    from rcvpose_amd.models.fcnresnet import ResFCNResNet152
+
+    shapes = json.load(open(os.path.join(golden_dir, "resfcn_state_dict_keys.json")))
+    sd = {k: torch.from_numpy(v) for k, v in fcn_weights.make_state_dict_numpy(shapes, seed=0).items()}
+    builder = fcn_engine.build_program_res(64, 96)
+    names = ["conv_up4.0", "conv_up3.0"]
+    for pattern, want_names in ((True, names), (r"conv_up[43]\.0|conv_up2_1", names + ["conv_up2_1"])):
+        eng = FcnEngine([sd], 64, 96, dtype=dtype, reuse_slots=False, arch="res", int8=pattern)
+        seg, rad = eng.forward(x)
+        assert sorted(s["conv"] for o, s in zip(eng.ops, builder.wspecs) if o["wq_off"]) == sorted(want_names)
+        for op, spec in zip(eng.ops, builder.wspecs):
+            if not op["wq_off"]:
+                continue
+            src, got = (eng.debug_slot(3, 0, op[k], (op["hin"], op["win"], op[c])).to(TORCH[dtype]) for k, c in (("src0", "c0"), ("dst", "cout")))
+            res = None if op["res"] < 0 else eng.debug_slot(3, 0, op["res"], (op["hin"], op["win"], op["cout"])).to(TORCH[dtype])
+            w, b = fcn_engine.fold_conv_bn(sd, spec, op["cout"])
+            weight = int8.quantize_weight(w[:, 0, 0] if op["ksize"] == 1 else w).to("cuda")
+            call = int8.matmul if op["ksize"] == 1 else int8.conv3x3
+            codes, scales = int8.quantize_tokens(src)
+            want = call(codes, scales, weight, bias=b.float().cuda(), residual=res, relu=bool(op["relu"]), dtype=TORCH[dtype]).double()
+            positive = int8.Int8Weight(weight.codes.abs(), weight.scales, weight.channels)
+            size = call(codes.abs(), scales, positive, bias=b.float().abs().cuda(), residual=None if res is None else res.float().abs(), dtype=torch.float32).double()
+            eps, diff = torch.finfo(TORCH[dtype]).eps, (got.double() - want).abs()
+            assert bool((diff <= 62 * 2.0 ** -24 * size * (1 + eps) + eps * want.abs() * (1 + eps) + 2.0 ** -24).all()), (spec["conv"], float(diff.max()))
+            assert float(want.abs().max()) > 0
+    m = ResFCNResNet152(3, 2).eval()
+    m.load_state_dict(sd)
+    m.set_compute_dtype(dtype, int8=pattern)
+    got = m(x)
+    eng = FcnEngine([sd], 64, 96, dtype=dtype, arch="res", int8=pattern)
+    ref = eng.forward(x)
+    assert torch.equal(got[0], ref[0][0]) and torch.equal(got[1], ref[1][0])
+    eng.set_option(16, 0)
+    plain = FcnEngine([sd], 64, 96, dtype=dtype, arch="res").forward(x)
+    off = eng.forward(x)
+    assert torch.equal(off[0], plain[0]) and torch.equal(off[1], plain[1]) and not torch.equal(ref[1], plain[1])
