@@ -1373,9 +1373,9 @@ __device__ __forceinline__ void d_bb_wide(AccHeader *hdr, const float *F, size_t
                 const float q[3] = {sb[0][li], sb[1][li], sb[2][li]};
                 const float tlo = sb[3][li], thi = sb[4][li];
                 const f32x2 thi2 = {thi, thi}, tlo2 = {tlo, tlo};
-                // dmin / dmax of both halves of one axis of parent u as float2 (v_pk_add_f32); max(e1^2, e2^2) = max(|e1|, |e2|)^2
+                // dmin / dmax of both halves of one axis of parent u as float2; max(e1^2, e2^2) = max(|e1|, |e2|)^2
                 // exactly (the |.| are free source modifiers).  r04: the squares are not formed on their own any more -- every sum
-                // they enter is one v_pk_fma_f32 (dmin * dmin + rest, rest - dmax * dmax): 16 multiplies less per four parents and
+                // they enter is one fused multiply-add (dmin * dmin + rest, rest - dmax * dmax): 16 multiplies less per four parents and
                 // point, and one rounding less per term, so the thresholds' float32 slack covers the sums as before
 #define RCV_BBW_AXIS(u, a, dn, dx)                                                                                          \
     {                                                                                                                       \

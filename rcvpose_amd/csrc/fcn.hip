@@ -107,8 +107,8 @@ __device__ __forceinline__ void x3_split(float v, H16 &hi, H16 &lo)
     lo = (H16)(v - (float)hi);
 }
 // eight consecutive channels as two 16-byte vectors.  Written on pairs: gfx950 converts two floats to packed halves in one
-// instruction (v_cvt_pk_f16_f32) and subtracts / adds two floats in one (v_pk_add_f32) -- 36 VALU instructions per eight
-// elements instead of 56 + 8 to pack; element for element the same IEEE operations as x3_split.
+// instruction (v_cvt_pk_f16_f32); element for element the same IEEE operations as x3_split.  (The build keeps the pairs' float32
+// operations scalar instructions.)
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 // (-DRCV_X3_SCALAR_HELPERS: the element-by-element forms, for an A-B check of the outputs' hash -- tools/fcn_hash.py)
 typedef _Float16 x3_h2 __attribute__((ext_vector_type(2)));
@@ -2436,9 +2436,11 @@ __device__ __forceinline__ float bilerp(float hy, float hx, float ly, float lx, 
 {
     const float t0 = __fmaf_rn(lx, p01, __fmul_rn(hx, p00));
     const float t1 = __fmaf_rn(lx, p11, __fmul_rn(hx, p10));
-    return __fmaf_rn(hy, t0, __fmul_rn(ly, t1));
+    float v = __fmaf_rn(hy, t0, __fmul_rn(ly, t1));
+    asm("" : "+v"(v));  // (a float32 number here: v_fma_mixlo_f16 would round the exact sum to half at once, in some callers and not in others)
+    return v;
 }
-// the same on eight channels, two per instruction (v_pk_mul_f32 / v_pk_fma_f32), in two stages so that the horizontal blends
+// the same on eight channels, written in pairs, in two stages so that the horizontal blends
 // of a source cell are formed once per destination column: element for element bilerp's operations
 __device__ __forceinline__ void bilerp8_rows(float hx, float lx, const float *p00, const float *p01, const float *p10, const float *p11,
                                              f32x2 *t0, f32x2 *t1)
@@ -4214,9 +4216,8 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? 3 : (CMID == 64 && !T3) ? 4 : 2
             if constexpr (FD == 2) asm volatile("s_waitcnt lgkmcnt(4)" : "+v"(ebi0), "+v"(ebi1), "+v"(esc0), "+v"(esc1));  // (at most FD tiles' fragments are newer: two reads each)
             else if constexpr (FD == 3) asm volatile("s_waitcnt lgkmcnt(6)" : "+v"(ebi0), "+v"(ebi1), "+v"(esc0), "+v"(esc1));
             else asm volatile("s_waitcnt lgkmcnt(8)" : "+v"(ebi0), "+v"(ebi1), "+v"(esc0), "+v"(esc1));
-            // (r06: pairs -- v_pk_fma_f32 / v_pk_add_f32 do two of the same IEEE operations per instruction: 19 % fewer vector instructions,
-            // no time gained.  tools/probe/mfma_valu_coissue_probe.hip says why: beside a SIMD's MFMAs an ordinary vector instruction
-            // costs ~1.6 cycles (mostly hidden), a packed-fp32 one ~7.7: it issues at half rate and is not hidden.)
+            // (written in pairs; the build keeps them scalar instructions.  Packed ones gained no time here: beside a SIMD's MFMAs an
+            // ordinary vector instruction costs ~1.6 cycles (mostly hidden), a packed one ~7.7.)
             evp[0] = __builtin_elementwise_fma(__builtin_shufflevector(accE[2 * t], accE[2 * t], 0, 1), __builtin_shufflevector(esc0, esc0, 0, 1), __builtin_shufflevector(ebi0, ebi0, 0, 1));
             evp[1] = __builtin_elementwise_fma(__builtin_shufflevector(accE[2 * t], accE[2 * t], 2, 3), __builtin_shufflevector(esc0, esc0, 2, 3), __builtin_shufflevector(ebi0, ebi0, 2, 3));
             break;

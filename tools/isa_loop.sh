@@ -3,7 +3,7 @@
 R=$(cd "$(dirname "$0")/.." && pwd)
 SRC=$R/rcvpose_amd/csrc/$1
 EXTRA=""; [ "$1" != "fcn.hip" ] && EXTRA="-ffp-contract=off"
-hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC $EXTRA -I$R/include -I$R/rcvpose_amd/csrc -S --cuda-device-only $SRC -o /tmp/isa_$$.s || exit 1
+hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -fPIC $EXTRA -I$R/include -I$R/rcvpose_amd/csrc -S --cuda-device-only $SRC -o /tmp/isa_$$.s || exit 1
 L=$(grep -n "^_Z.*$2.*:" /tmp/isa_$$.s | head -1 | cut -d: -f1)
 awk -v L=$L 'NR>=L{print} NR>L && /s_endpgm/{exit}' /tmp/isa_$$.s > /tmp/kernel.s
 D=${3:-3}

@@ -6,7 +6,7 @@ SRC=${1:-$R/rcvpose_amd/csrc/fcn_x3.hip}
 shift
 EXTRA=""
 case "$SRC" in *accumulator.hip|*pose.hip|*icp.hip) EXTRA="-ffp-contract=off";; esac
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -I$R/include -I$R/rcvpose_amd/csrc $EXTRA "$@" -c $SRC -o /tmp/kres_$$.o \
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -fPIC -I$R/include -I$R/rcvpose_amd/csrc $EXTRA "$@" -c $SRC -o /tmp/kres_$$.o \
     -Rpass-analysis=kernel-resource-usage 2>&1 | python3 -c '
 import re, sys
 cur = None

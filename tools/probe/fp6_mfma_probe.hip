@@ -1,5 +1,5 @@
 // v_mfma_scale_f32_16x16x128_f8f6f4 with fp6 (e2m3) operands on gfx950: operand layout, scale semantics, zero-padded blocks, rate.
-//   hipcc --offload-arch=gfx950 -O2 tools/probe/fp6_mfma_probe.hip -o tools/probe/fp6_mfma_probe && tools/probe/fp6_mfma_probe
+//   hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops tools/probe/fp6_mfma_probe.hip -o tools/probe/fp6_mfma_probe && tools/probe/fp6_mfma_probe
 // Assumed (checked here against a host emulation with exactly representable data):
 //   lane l holds row (A) / column (B) l & 15 and the 32 K elements of block l >> 4 (k = 32 * (l >> 4) + j), element j in bits
 //   [6j, 6j + 6) of its six operand registers; e2m3 = sign | 2-bit exponent (bias 1) | 3-bit mantissa; the scale operand's

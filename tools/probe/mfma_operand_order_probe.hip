@@ -3,7 +3,7 @@
 // same registers.)  20 accumulator tiles acc[5][4], operands a[5] (tile rows), b[4] (tile columns), v_mfma_f32_16x16x32_f16; cycles per
 // MFMA (s_memtime) for the four (role, loop order) combinations, at one and at two waves per SIMD, with and without the three-pass
 // hi/lo structure of the split engine.
-//   hipcc --offload-arch=gfx950 -O3 tools/probe/mfma_operand_order_probe.hip -o /tmp/moo && /tmp/moo
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/probe/mfma_operand_order_probe.hip -o /tmp/moo && /tmp/moo
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdlib.h>

@@ -5,7 +5,7 @@
 // sustained TFLOP/s and the implied clock (flops / (1024 flop per cycle and SIMD x 1024 SIMDs)), at one and two waves per SIMD, with
 // independent accumulators (4 for 16x16, 2 for 32x32: the same 16 accumulator registers) and, for the split engine's pattern, chains of
 // three dependent MFMAs.
-//   hipcc --offload-arch=gfx950 -O3 tools/probe/mfma_shape_rate_probe.hip -o /tmp/msr && /tmp/msr
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/probe/mfma_shape_rate_probe.hip -o /tmp/msr && /tmp/msr
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));

@@ -1,6 +1,6 @@
 // v_fma_mix_f32 against convert-then-add on gfx950: (float)a + (float)b for all 65536 half patterns a x 4096 patterns b (both
 // halves of a dword), and v - (float)h for 2^20 float patterns v; NaN results compare as equal.  Expected: 0 mismatches.
-//   hipcc --offload-arch=gfx950 -O2 tools/probe/mix_probe.hip -o tools/probe/mix_probe && tools/probe/mix_probe
+//   hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops tools/probe/mix_probe.hip -o tools/probe/mix_probe && tools/probe/mix_probe
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 __device__ __forceinline__ float mix_add_lo(unsigned a, unsigned b) { float r; asm("v_fma_mix_f32 %0, %1, 1.0, %2 op_sel:[0,0,0] op_sel_hi:[1,0,1]" : "=v"(r) : "v"(a), "v"(b)); return r; }

@@ -1,5 +1,5 @@
 // Does MODE.FP16_OVFL (bit 23 of the MODE register) make v_cvt_pk_f16_f32 / v_cvt_f16_f32 saturate on gfx950?
-//   hipcc --offload-arch=gfx950 -O2 tools/probe/ovfl_probe.hip -o tools/probe/ovfl_probe && tools/probe/ovfl_probe
+//   hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops tools/probe/ovfl_probe.hip -o tools/probe/ovfl_probe && tools/probe/ovfl_probe
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <math.h>

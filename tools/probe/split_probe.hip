@@ -1,5 +1,5 @@
 // split_probe.hip -- numerics probe for the split-precision (fp16 hi/lo, three MFMAs per product) convolution mode.
-// Standalone: hipcc --offload-arch=gfx950 -O2 -o split_probe split_probe.hip && ./split_probe
+// Standalone: hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops -o split_probe split_probe.hip && ./split_probe
 //   1. do fp16 MFMA operands keep subnormals?
 //   2. error of a K-long dot product against float64: fp32 MFMA chain, plain fp16 MFMA, hi/lo split (with and without
 //      power-of-two weight scaling).
