@@ -105,3 +105,15 @@ def test_every_source_is_compiled_without_packed_float32_instructions():
         for line in open(path):
             if "hipcc" in line and "--offload-arch" in line and "-shared" not in line:
                 assert "-packed-fp32-ops" in line, path
+
+
+def test_build_compiles_whatever_is_built_already(monkeypatch):
+    import __graft_entry__
+    from oracle import cpu_oracle
+    from rcvpose_amd import build
+
+    seen = []
+    monkeypatch.setattr(build, "build_library", lambda force=False, verbose=False: seen.append(force) or build.LIB)
+    monkeypatch.setattr(cpu_oracle, "build", lambda *a, **kw: None)
+    __graft_entry__.build()
+    assert seen == [True]
