@@ -995,7 +995,7 @@ Plan plan_product(long long rows, int K, int Cout, int taps, int groups)
     // (two 16-channel tiles per workgroup share the tokens once all CUs are busy: 32 x 1024 -> 8192 5.2 / 6.1, 64 x 2048 -> 8192 9.8 / 12.5,
     // but 32 x 4096 -> 4096 10.6 / 8.9)
     pl.wide_direct = taps == 1 && rows > 16 && small >= 512;
-    const long long token_bytes = (pl.wide_direct ? tiles(64, 32) : small) * std::min(rows, 64LL) * taps * ((K + 63) & ~63);
+    const double token_bytes = (double)(pl.wide_direct ? tiles(64, 32) : small) * std::min(rows, 64LL) * taps * ((K + 63) & ~63);
     const bool few = small <= 320 || (small <= 640 && (taps == 9 || token_bytes <= 16000000));
     // (windows whose rows lie whole cache lines apart read few of the cache's channels at a time: 1 x 30 x 40, 256 -> 256 15.2 / 14.0, but
     // 3 x 21 x 18, 355 -> 208 9.7 / 14.4)
@@ -1168,6 +1168,11 @@ using namespace rcv;
 namespace {
 constexpr long long I8_MAX_ROWS = 1LL << 32;
 constexpr int I8_MAX_K = 131071, I8_MAX_COUT = 1 << 20;
+// Sizes that check_args takes: what plan_product computes of them stays within its integers.
+bool countable(long long rows, int channels, int out_channels)
+{
+    return rows > 0 && rows <= I8_MAX_ROWS && channels > 0 && channels <= I8_MAX_K && out_channels > 0 && out_channels <= I8_MAX_COUT;
+}
 bool float_type(int dtype) { return dtype == RCV_F32 || dtype == RCV_BF16 || dtype == RCV_F16; }
 
 int check_args(const rcv_i8_args *a, int taps, I8Product &p)
@@ -1216,12 +1221,12 @@ int rcv_i8_quantize_tokens(const void *x0_dev, long long pitch0, int c0, const v
 
 size_t rcv_i8_matmul_workspace_bytes(long long rows, int channels, int out_channels)
 {
-    return rows > 0 && channels > 0 && out_channels > 0 ? i8_product_workspace(rows, channels, out_channels, 1, 1) : 0;
+    return countable(rows, channels, out_channels) ? i8_product_workspace(rows, channels, out_channels, 1, 1) : 0;
 }
 
 size_t rcv_i8_conv3x3_workspace_bytes(long long rows, int channels, int out_channels)
 {
-    return rows > 0 && channels > 0 && out_channels > 0 ? i8_product_workspace(rows, channels, out_channels, 9, 1) : 0;
+    return countable(rows, channels, out_channels) ? i8_product_workspace(rows, channels, out_channels, 9, 1) : 0;
 }
 
 int rcv_i8_matmul(const rcv_i8_args *args, void *ws, size_t ws_bytes, void *stream)

@@ -298,3 +298,11 @@ def test_pipeline_refuses_int8_for_an_engine_that_is_built():
 
     with pytest.raises(ValueError, match="int8"):
         FramePipeline([{}], 64, 96, dtype="bf16", fcn=object(), int8=True)
+
+
+@pytest.mark.parametrize("name", ["rcv_i8_matmul", "rcv_i8_conv3x3"])
+@pytest.mark.parametrize("rows, k, n", [(5, 2 ** 31 - 1, 64), (5, 131072, 64), (2 ** 62, 4096, 64), ((1 << 32) + 1, 4096, 64), (5, 4096, 2 ** 31 - 1),
+                                        (5, 4096, (1 << 20) + 1), (-5, 4096, 64), (5, -4096, 64), (5, 4096, -64)])
+def test_sizes_that_are_refused_need_no_workspace(name, rows, k, n):
+    """(What the plan of such a size would need cannot be counted in its integers.)"""
+    assert getattr(_hip.load_library(), name + "_workspace_bytes")(rows, k, n) == 0
