@@ -600,7 +600,8 @@ class FcnEngine:
 
         x: the static input tensor (refill it in place before a replay); returns (graph, seg, radial): `graph.replay()`
         re-runs the captured launches on the current stream and leaves the result in seg / radial.  Per-op profiling must
-        be off; the layer program, options and batch size are frozen into the graph."""
+        be off; the layer program, options and batch size are frozen into the graph.  The graph keeps the engine's workspace of the
+        capture (`graph.workspace`); an engine's graphs and forwards that share one run one after the other."""
         import torch
 
         B = x.shape[0]
@@ -616,6 +617,7 @@ class FcnEngine:
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             self.forward(x, out=out)
+        graph.workspace = self._ws  # (a forward of a larger batch takes another: the graph's launches still write here)
         return graph, out[0], out[1]
 
     def debug_stage(self, B, g, name):

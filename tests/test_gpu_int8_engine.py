@@ -266,3 +266,22 @@ def test_res_network(golden_dir, x, dtype):
     plain = FcnEngine([sd], 64, 96, dtype=dtype, arch="res").forward(x)
     off = eng.forward(x)
     assert torch.equal(off[0], plain[0]) and torch.equal(off[1], plain[1]) and not torch.equal(ref[1], plain[1])
+
+
+@pytest.mark.parametrize("dtype, int8_layers", [("bf16", False), ("fp16", True)])
+def test_a_graph_keeps_its_workspace(sds, x, dtype, int8_layers):
+    """A forward of a larger batch gives the engine another workspace; what takes the first one's memory must not be written by a replay."""
+    eng = FcnEngine(sds, 64, 96, dtype=dtype, int8=int8_layers)
+    graph, seg, rad = eng.capture(x[:1])
+    assert graph.workspace is eng.workspace(1)
+    want = [t.clone() for t in eng.forward(x[:1])]
+    size = eng.workspace(1).numel()
+    eng.forward(x)
+    assert graph.workspace is not eng.workspace(1)
+    others = [torch.full((size,), 77, dtype=torch.uint8, device="cuda") for _ in range(3)]
+    for _ in range(3):
+        seg.zero_(), rad.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(seg, want[0]) and torch.equal(rad, want[1])
+        assert all(int((t != 77).sum()) == 0 for t in others)
