@@ -574,3 +574,8 @@ def test_rows_farther_apart_than_the_kernels_take(c):
 def test_matmul_of_many_rows_with_a_residual(k, dtype):
     """Both sides of the sums from which the widest tiles take odd rows and residuals."""
     test_matmul(12301, k, 1025, dtype)
+
+
+def test_a_float16_token_has_the_same_product_in_any_batch():
+    """float16 too: the float32 sum is rounded before it is rounded to half, in every kernel."""
+    test_a_token_has_the_same_product_in_any_batch(torch.float16)
