@@ -117,3 +117,15 @@ def test_build_compiles_whatever_is_built_already(monkeypatch):
     monkeypatch.setattr(cpu_oracle, "build", lambda *a, **kw: None)
     __graft_entry__.build()
     assert seen == [True]
+
+
+@pytest.mark.parametrize("script", ["ab_build.sh", "variant_build.sh"])
+def test_variant_builds_link_every_unit(script):
+    """A library without one of the units does not load."""
+    from rcvpose_amd import build
+
+    link = [line for line in open(os.path.join(ROOT, "tools", script)) if "hipcc" in line and "-shared" in line]
+    assert len(link) == 1
+    for source in build.SOURCES:
+        if source != "fcn_x3.hip":  # (the unit that the script builds itself)
+            assert "$B/" + source.replace(".hip", ".o") in link[0].split(), source

@@ -8,6 +8,6 @@ mkdir -p $R/tools/probe/ab
 python -m rcvpose_amd.build > /dev/null || exit 1
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -fPIC -I$R/include -I$R/rcvpose_amd/csrc "$@" -c $R/rcvpose_amd/csrc/fcn_x3.hip -o $R/tools/probe/ab/fcn_x3_$NAME.o || exit 1
 B=$R/rcvpose_amd/build
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o $R/tools/probe/ab/lib_$NAME.so $B/core.o $B/accumulator.o $B/fcn.o $B/fcn_f16.o $R/tools/probe/ab/fcn_x3_$NAME.o $B/pose.o $B/icp.o || exit 1
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o $R/tools/probe/ab/lib_$NAME.so $B/core.o $B/accumulator.o $B/fcn.o $B/fcn_f16.o $R/tools/probe/ab/fcn_x3_$NAME.o $B/pose.o $B/icp.o $B/int8.o || exit 1
 rm -f $R/tools/probe/ab/fcn_x3_$NAME.o
 echo $R/tools/probe/ab/lib_$NAME.so
