@@ -54,6 +54,7 @@ class DenseFCNResNet152(nn.Module):
     # width, number of plain bottlenecks after the projecting one, stride of the projecting one
     _encoder = ((64, 2, 1), (128, 7, 2), (256, 35, 2), (512, 2, 2))
     _arch = "dense"
+    int8 = False  # (of modules that were saved whole before they had it)
 
     def __init__(self, input_channels=3, output_channels=2):
         super().__init__()
@@ -82,7 +83,6 @@ class DenseFCNResNet152(nn.Module):
         # "fp32": exact-fp32 MFMA kernels (v_mfma_f32_16x16x4_f32)
         # "bf16" / "fp16": 16-bit storage / fp32 accumulate (throughput modes outside the 1e-4 tolerance)
         self.compute_dtype = "f16x3"
-        self.int8 = False
         self._engine = None
         self._engine_key = None
 
@@ -153,6 +153,5 @@ class ResFCNResNet152(DenseFCNResNet152):
         self.conv7 = _decoder_stage(128, 64)
         self.conv8 = nn.Conv2d(64, output_channels, kernel_size=1, stride=1)
         self.compute_dtype = "f16x3"
-        self.int8 = False
         self._engine = None
         self._engine_key = None

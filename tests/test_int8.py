@@ -306,3 +306,17 @@ def test_pipeline_refuses_int8_for_an_engine_that_is_built():
 def test_sizes_that_are_refused_need_no_workspace(name, rows, k, n):
     """(What the plan of such a size would need cannot be counted in its integers.)"""
     assert getattr(_hip.load_library(), name + "_workspace_bytes")(rows, k, n) == 0
+
+
+def test_a_module_saved_before_it_had_int8_layers_runs_without():
+    import copy
+
+    from rcvpose_amd.models.fcnresnet import DenseFCNResNet152, ResFCNResNet152
+
+    for cls in (DenseFCNResNet152, ResFCNResNet152):
+        state = cls(3, 2).__dict__.copy()
+        state.pop("int8", None)
+        m = cls.__new__(cls)
+        m.__setstate__(state)
+        assert m.int8 is False and m.compute_dtype == "f16x3"
+        assert copy.copy(m.set_compute_dtype("bf16", int8=True)).int8 is True
