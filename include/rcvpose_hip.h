@@ -423,7 +423,7 @@ int rcv_fcn_set_profiling(rcv_fcn *h, int enable);
  * 7.9 against 7.3 ms.
  * key 16 (default 1, RCV_BF16 / RCV_F16): 8-bit integer arithmetic for the ops whose wq_off names an int8 copy of their weights: the op's
  * source pixels are quantised (rcv_i8_quantize_tokens, one scale per pixel over the concatenated channels) into scratch behind the
- * activation slots, then multiplied as integers (rcv_i8_matmul / rcv_i8_conv3x3).  The key only ENABLES the form, an op takes it when it has
+ * activation slots, then multiplied as integers (rcv_i8_matmul / rcv_i8_conv3x3, its taps in one order whatever the batch).  The key only ENABLES the form, an op takes it when it has
  * the copy, and such an op joins none of the fused kernels.  0: the 16-bit kernels (maps as without the copies). */
 int rcv_fcn_set_option(rcv_fcn *h, int key, int value);
 int rcv_fcn_get_profile(rcv_fcn *h, double *conv_ms, double *other_ms, double *conv_flop);

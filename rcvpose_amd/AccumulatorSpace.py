@@ -514,7 +514,7 @@ def estimate_6d_pose_lm(opts, return_details=False):
             # equal batches: the device pipeline runs whole batches, so 128 frames travel as 43 + 43 + 42, not as 53 + 53 + 22 with
             # 31 padded frames of wasted work
             # (the default of 53 is tuned for one MI355X with 288 GB: on a smaller or shared device the workspaces of a batch may not
-            # fit -- halve the batch until they do; results do not depend on it, but with int8 layers: FcnEngine)
+            # fit -- halve the batch until they do; results do not depend on it)
             # The engine is built ONCE; the batch is then sized from the free device memory and the byte counts of a batch's
             # workspaces (nothing is allocated to find out), and an allocation that fails all the same -- another process took the
             # memory in between -- is retried with half the batch OUTSIDE the except block (inside it the traceback still holds the
@@ -554,8 +554,7 @@ def estimate_6d_pose_lm(opts, return_details=False):
             # host threads, each on its own HIP stream (a frame's evaluation is a chain of small launches and a few
             # synchronisations: one thread spends it waiting, sixteen overlap).  A frame's maps and keypoints do not
             # depend on the batch it travels in (tests/test_gpu_fcn_x3.py::test_x3_groups_and_batch), so the results are those
-            # of the frame-by-frame loop of the reference (:553-659).  (opts.int8 is the exception: its windows are added in an
-            # order that the batch size decides.)
+            # of the frame-by-frame loop of the reference (:553-659).
             from concurrent.futures import ThreadPoolExecutor
 
             from PIL import Image

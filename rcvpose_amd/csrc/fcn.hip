@@ -5154,7 +5154,7 @@ I8Scratch i8_scratch(const rcv_fcn *h, const rcv_op &o, int B)
     s.scales = align_up((size_t)rows * h->groups * align_up((size_t)C, 16), 256);
     s.partial = align_up(s.scales + (size_t)rows * h->groups * 4, 256);
     // (a bound that grows with the batch: the parts themselves come and go with it, and a workspace of the largest batch serves the others)
-    s.bytes = align_up(s.partial + i8_product_workspace_most(rows, C, o.cout, o.ksize * o.ksize, h->groups), 256);
+    s.bytes = align_up(s.partial + i8_product_workspace_most(rows, C, o.cout, o.ksize * o.ksize, h->groups, true), 256);
     return s;
 }
 size_t i8_scratch_bytes(const rcv_fcn *h, int B)
@@ -5201,6 +5201,7 @@ int run_int8(rcv_fcn *h, const rcv_op &o, int B, char *ws, const std::vector<siz
     p.rows = rows;
     p.K = C; p.kp = i8_kp(C); p.Cout = o.cout; p.taps = o.ksize * o.ksize; p.H = o.hin; p.W = o.win;
     p.relu = o.relu; p.out_dtype = h->dtype; p.groups = h->groups; p.range = h->range_dev;
+    p.one_order = true;  // (an image's maps do not depend on its batch, as in every other op)
     return i8_product(p, scratch + s.partial, s.bytes - s.partial, st);
 }
 

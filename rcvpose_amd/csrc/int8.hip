@@ -979,9 +979,11 @@ struct Plan {
 
 // The times beside the rules are microseconds of one call in a graph, bfloat16 out; M x K -> N for a product, images x height x width, K -> N
 // for a window.
-Plan plan_product(long long rows, int K, int Cout, int taps, int groups)
+Plan plan_product(long long rows, int K, int Cout, int taps, int groups, bool one_order)
 {
     Plan pl{Plan::SQUARE, 1, 0, false};
+    // k_i8_tile adds the nine taps one after the other, whatever its tiles; k_i8_direct and divided sums scale and add other pieces of them.
+    const bool whole = one_order && taps == 9;
     const int steps = taps * ((K + 127) / 128);
     auto tiles = [&](int bm, int bn) { return ((rows + bm - 1) / bm) * ((Cout + bn - 1) / bn) * groups; };
 
@@ -999,7 +1001,7 @@ Plan plan_product(long long rows, int K, int Cout, int taps, int groups)
     const bool few = small <= 320 || (small <= 640 && (taps == 9 || token_bytes <= 16000000));
     // (windows whose rows lie whole cache lines apart read few of the cache's channels at a time: 1 x 30 x 40, 256 -> 256 15.2 / 14.0, but
     // 3 x 21 x 18, 355 -> 208 9.7 / 14.4)
-    if (rows <= 4 || (token_bytes <= (taps == 9 && K % 128 == 0 ? 42000000 : 60000000) && (rows <= 64 || few))) {
+    if (!whole && (rows <= 4 || (token_bytes <= (taps == 9 && K % 128 == 0 ? 42000000 : 60000000) && (rows <= 64 || few)))) {
         pl.kind = Plan::DIRECT;
         // Workgroups divide a long sum while CUs are free.  In 1 / 2 / 4 / 8 parts: 1 x 16384 -> 512 11.7 / 9.4 / 7.7 / 7.5, 1 x 4096 -> 512
         // 5.3 / 6.1 / 6.2 / 7.0, 1 x 8192 -> 64 7.3 / 7.0 / 6.8, 45 x 2343 -> 758 5.9 / 7.1, 64 x 4096 -> 512 12.0 / 9.9 / 8.4; windows
@@ -1026,7 +1028,7 @@ Plan plan_product(long long rows, int K, int Cout, int taps, int groups)
             // 256 x 128 / 128 x 128: 53 x 30 x 40, 2048 -> 512 551 / 663, 8 x 60 x 80, 128 -> 128 20 / 25; one round of either:
             // 12 x 15 x 20, 2048 -> 1024 106 / 83
             pl.kind = Plan::TALL;
-        if (pl.kind == Plan::SQUARE) {
+        if (pl.kind == Plan::SQUARE && !whole) {
             // Few tiles of a long sum: workgroups divide it while the CUs hold them at once.  In 1 / 3 / 9 parts (taps): 1 x 15 x 20,
             // 2048 -> 1024 67 / 30 / 23, 1 x 30 x 40, 2048 -> 512 68 / 32 / 33, 3 x 28 x 43, 717 -> 127 30 / 19 / 24, 1 x 60 x 80,
             // 1024 -> 256 39 / 27 / 44, 512 -> 256 23 / 24 / 35, 128 -> 256 13 / 21 / 37, 2 x 69 x 54, 488 -> 61 24 / 17 / 28,
@@ -1120,7 +1122,7 @@ template <typename T, int TAPS> int launch_taps(const I8Product &p, const Plan &
 
 template <typename T> int launch_product(const I8Product &p, void *ws, hipStream_t st)
 {
-    const Plan pl = plan_product(p.rows, p.K, p.Cout, p.taps, p.groups);
+    const Plan pl = plan_product(p.rows, p.K, p.Cout, p.taps, p.groups, p.one_order);
     return p.taps == 9 ? launch_taps<T, 9>(p, pl, ws, st) : launch_taps<T, 1>(p, pl, ws, st);
 }
 
@@ -1135,17 +1137,17 @@ int i8_quantize(const void *x0, long long pitch0, int c0, const void *x1, long l
     return launch_quantize<_Float16>(x0, pitch0, c0, x1, pitch1, c1, rows, codes, codes_pitch, scales, st);
 }
 
-size_t i8_product_workspace(long long rows, int K, int Cout, int taps, int groups)
+size_t i8_product_workspace(long long rows, int K, int Cout, int taps, int groups, bool one_order)
 {
-    return rows > 0 ? plan_product(rows, K, Cout, taps, groups).bytes : 0;
+    return rows > 0 ? plan_product(rows, K, Cout, taps, groups, one_order).bytes : 0;
 }
 
 // plan_product divides a sum while its tiles (of at most 128 x 128) times its parts are at most 256, by channels into eight parts or parts of
 // at least eight steps, by taps into nine.
-size_t i8_product_workspace_most(long long rows, int K, int Cout, int taps, int groups)
+size_t i8_product_workspace_most(long long rows, int K, int Cout, int taps, int groups, bool one_order)
 {
     constexpr long long ALL = 256 * 128 * 128 * 4;
-    if (rows <= 0) return 0;
+    if (rows <= 0 || (taps == 9 && one_order)) return 0;
     const long long parts = taps == 9 ? 9 : std::max(8, (K + 127) / 128 / 8), row = parts * groups * ((Cout + 3) / 4) * 16;
     return (size_t)(rows > ALL / row ? ALL : rows * row);
 }
@@ -1153,7 +1155,7 @@ size_t i8_product_workspace_most(long long rows, int K, int Cout, int taps, int 
 int i8_product(const I8Product &p, void *ws, size_t ws_bytes, hipStream_t st)
 {
     if (p.rows == 0) return RCV_OK;
-    const size_t need = i8_product_workspace(p.rows, p.K, p.Cout, p.taps, p.groups);
+    const size_t need = i8_product_workspace(p.rows, p.K, p.Cout, p.taps, p.groups, p.one_order);
     if (need && (ws_bytes < need || !ws)) return RCV_E_WORKSPACE;
     if ((uintptr_t)ws % 16) return RCV_E_INVALID;
     if (p.out_dtype == RCV_F32) return launch_product<float>(p, ws, st);
@@ -1221,12 +1223,12 @@ int rcv_i8_quantize_tokens(const void *x0_dev, long long pitch0, int c0, const v
 
 size_t rcv_i8_matmul_workspace_bytes(long long rows, int channels, int out_channels)
 {
-    return countable(rows, channels, out_channels) ? i8_product_workspace(rows, channels, out_channels, 1, 1) : 0;
+    return countable(rows, channels, out_channels) ? i8_product_workspace(rows, channels, out_channels, 1, 1, false) : 0;
 }
 
 size_t rcv_i8_conv3x3_workspace_bytes(long long rows, int channels, int out_channels)
 {
-    return countable(rows, channels, out_channels) ? i8_product_workspace(rows, channels, out_channels, 9, 1) : 0;
+    return countable(rows, channels, out_channels) ? i8_product_workspace(rows, channels, out_channels, 9, 1, false) : 0;
 }
 
 int rcv_i8_matmul(const rcv_i8_args *args, void *ws, size_t ws_bytes, void *stream)

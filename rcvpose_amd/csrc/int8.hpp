@@ -15,14 +15,15 @@ struct I8Product {
     long long code_gs, weight_scale_gs, bias_gs, residual_gs, out_gs;  // (the token scales' group stride is code_gs as well)
     int K, kp, Cout, taps, H, W;
     int relu, out_dtype, groups;
+    bool one_order;                     // taps = 9: a window's bits do not depend on rows or groups (undivided sums)
     unsigned *range;                    // RCV_F16 engines: the sticky range-flag word, or null
 };
 
 int i8_quantize(const void *x0, long long pitch0, int c0, const void *x1, long long pitch1, int c1, int dtype, long long rows,
                 int8_t *codes, long long codes_pitch, float *scales, hipStream_t st);
-size_t i8_product_workspace(long long rows, int K, int Cout, int taps, int groups);
+size_t i8_product_workspace(long long rows, int K, int Cout, int taps, int groups, bool one_order);
 // No less than i8_product_workspace of these or of fewer rows.
-size_t i8_product_workspace_most(long long rows, int K, int Cout, int taps, int groups);
+size_t i8_product_workspace_most(long long rows, int K, int Cout, int taps, int groups, bool one_order);
 int i8_product(const I8Product &p, void *ws, size_t ws_bytes, hipStream_t st);
 
 constexpr int I8_KP = 128;  // weight rows are padded with zeros to a multiple of this many codes per tap

@@ -33,8 +33,7 @@ def build_parser():
                         "cent faster, keypoints a few voxels less exact")
     p.add_argument('--frames_per_step', type=int, default=53,
                    help="frames of a class that travel through the device pipeline together (LINEMOD loop with checkpoints; default: "
-                        "bench.py's batch); results do not depend on it (with --int8 they may: float32 sums are added in an order that the batch decides, "
-                        "and maps can differ by some 1e-2 of their range at a few pixels)")
+                        "bench.py's batch); results do not depend on it")
     p.add_argument('--eval_threads', type=int, default=default_eval_threads(),
                    help="host threads (one HIP stream each) for the per-frame Horn / ADD(-S) / ICP evaluation of a batch")
     return p

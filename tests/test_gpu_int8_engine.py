@@ -173,34 +173,29 @@ def test_a_workspace_of_a_larger_batch_serves_a_smaller_one(sds, x, dtype, int8)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
-def test_an_image_alone_and_among_others(sds, x, dtype):
-    """A batch of another size may divide a window's sum otherwise.  The first int8 layer has the same source in both, bit for bit; its two
-    results are within 31 roundings of float32 (nine taps, up to sixteen partial sums, scale, bias, residual) of one real number each,
-    and are then rounded by at most half a step of the stored type.  What the layers behind make of a moved step is printed."""
-    engines = [FcnEngine(sds[:1], 64, 96, dtype=dtype, reuse_slots=False, int8=True) for _ in range(2)]
-    batches = (1, 17)
-    many = x[:1].repeat(17, 1, 1, 1)
-    many[1:] *= 0.7
-    maps = [eng.forward(many[:b])[1][0, 0, 0] for eng, b in zip(engines, batches)]
-    builder = fcn_engine.build_program(64, 96)
-    first = next(i for i, op in enumerate(engines[0].ops) if op["wq_off"])
-    op, spec = engines[0].ops[first], builder.wspecs[first]
-    assert spec["conv"] == "conv6" and op["src1"] < 0 and op["res"] < 0
-    src = [eng.debug_slot(b, 0, op["src0"], (op["hin"], op["win"], op["c0"]))[0] for eng, b in zip(engines, batches)]
-    out = [eng.debug_slot(b, 0, op["dst"], (op["hout"], op["wout"], op["cout"]))[0].double() for eng, b in zip(engines, batches)]
-    assert torch.equal(src[0], src[1])
-    w, bias = fcn_engine.fold_conv_bn(sds[0], spec, op["cout"])
-    weight = int8.quantize_weight(w).to("cuda")
-    codes, scales = int8.quantize_tokens(src[0][None].to(TORCH[dtype]))
-    size = int8.conv3x3(codes.abs(), scales, int8.pack_codes(weight.codes[:, :, :weight.channels].abs().reshape(w.shape), weight.scales),
-                        bias=bias.float().abs().cuda(), dtype=torch.float32)[0].double()
-    eps = torch.finfo(TORCH[dtype]).eps
-    diff = (out[0] - out[1]).abs()
-    assert bool((diff <= 62 * 2.0 ** -24 * size * (1 + eps) + eps * out[1].abs() * (1 + eps) + 2.0 ** -24).all()), float(diff.max())
-    assert float(out[1].abs().max()) > 0
-    print("%s: image alone and among 17: radial maps differ by %.2e of their range" % (dtype, float((maps[0] - maps[1]).abs().max() / maps[1].abs().max())))
-    again = [eng.forward(many[:b])[1][0, 0, 0] for eng, b in zip(engines, batches)]
-    assert torch.equal(again[0], maps[0]) and torch.equal(again[1], maps[1])  # (in one batch size: the same bits)
+@pytest.mark.parametrize("int8_layers", [True, r"conv6|conv_up[54321]\.0|conv7\.0|block[234](up)?(\.\d)?\.conv[123]"])
+def test_an_image_alone_and_among_others(sds, x, dtype, int8_layers):
+    """An image's maps are the same bits in any batch and beside any number of networks, as with 16-bit layers."""
+    eng = FcnEngine(sds, 64, 96, dtype=dtype, int8=int8_layers)
+    alone = [t.clone() for t in eng.forward(x[:1])]
+    many = x[:1].repeat(57, 1, 1, 1)
+    many[1:] *= torch.linspace(0.5, 1.5, 56, device="cuda").view(56, 1, 1, 1)
+    for b in (2, 3, 8, 17, 57):
+        got = eng.forward(many[:b])
+        assert torch.equal(got[0][:, :1], alone[0]) and torch.equal(got[1][:, :1], alone[1]), b
+    single = FcnEngine(sds[1:], 64, 96, dtype=dtype, int8=int8_layers).forward(many[:1])
+    assert torch.equal(single[0][0], alone[0][1]) and torch.equal(single[1][0], alone[1][1])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_a_frame_alone_and_among_others(sds, dtype):
+    """The same at 480 x 640, where one frame's windows used to be added in another order than eight frames'."""
+    frames = torch.randn(8, 3, 480, 640, generator=torch.Generator().manual_seed(1)).cuda()
+    eng = FcnEngine(sds, 480, 640, dtype=dtype, int8=True)
+    alone = [t.clone() for t in eng.forward(frames[:1])]
+    for b in (2, 8):
+        got = eng.forward(frames[:b])
+        assert torch.equal(got[0][:, :1], alone[0]) and torch.equal(got[1][:, :1], alone[1]), b
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
