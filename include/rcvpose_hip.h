@@ -452,7 +452,7 @@ int rcv_i8_quantize_tokens(const void *x0_dev, long long pitch0, int c0, const v
  *
  * rcv_i8_matmul: one tap, m(tap) = m.  rcv_i8_conv3x3: the nine taps of a 3x3 window with zero padding and stride 1 over images of
  * height x width tokens (rows = images * height * width, row-major).  Sums of codes are exact 32-bit integers.  What follows is float32,
- * each step rounded: the sum's conversion (whole numbers above 2^24), its token scale, the weight scale and the bias in one step, the
+ * each step rounded, and infinite where it leaves the range: the sum's conversion (whole numbers above 2^24), its token scale, the weight scale and the bias in one step, the
  * residual; the result is then rounded to out_dtype.  rcv_i8_conv3x3 converts and scales the sum of a tap, or of a run of a tap's channels,
  * and adds these in float32 in an order that the sizes alone decide: two calls of one size give the same bits, a window among more or
  * fewer images may differ in its float32 sum's last bits, and no result is off by more than 31 roundings of the sum of the magnitudes that
