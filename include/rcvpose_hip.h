@@ -423,8 +423,8 @@ int rcv_fcn_set_profiling(rcv_fcn *h, int enable);
  * 7.9 against 7.3 ms.
  * key 16 (default 1, RCV_BF16 / RCV_F16): 8-bit integer arithmetic for the ops whose wq_off names an int8 copy of their weights: the op's
  * source pixels are quantised (rcv_i8_quantize_tokens, one scale per pixel over the concatenated channels) into scratch behind the
- * activation slots, then multiplied as integers (rcv_i8_matmul / rcv_i8_conv3x3, its taps in one order whatever the batch).  The key only ENABLES the form, an op takes it when it has
- * the copy, and such an op joins none of the fused kernels.  0: the 16-bit kernels (maps as without the copies). */
+ * activation slots, then multiplied as integers (rcv_i8_matmul / rcv_i8_conv3x3, its taps in one order whatever the batch).  The key only
+ * ENABLES the form, an op takes it when it has the copy, and such an op joins none of the fused kernels.  0: the 16-bit kernels (maps as without the copies). */
 int rcv_fcn_set_option(rcv_fcn *h, int key, int value);
 int rcv_fcn_get_profile(rcv_fcn *h, double *conv_ms, double *other_ms, double *conv_flop);
 /* Per-op device times (ms) of the last profiled forward; ms_out has room for n_ops doubles. */
@@ -452,11 +452,12 @@ int rcv_i8_quantize_tokens(const void *x0_dev, long long pitch0, int c0, const v
  *
  * rcv_i8_matmul: one tap, m(tap) = m.  rcv_i8_conv3x3: the nine taps of a 3x3 window with zero padding and stride 1 over images of
  * height x width tokens (rows = images * height * width, row-major).  Sums of codes are exact 32-bit integers.  What follows is float32,
- * each step rounded, and infinite where it leaves the range: the sum's conversion (whole numbers above 2^24), its token scale, the weight scale and the bias in one step, the
- * residual; the result is then rounded to out_dtype.  rcv_i8_conv3x3 converts and scales the sum of a tap, or of a run of a tap's channels,
- * and adds these in float32 in an order that the sizes alone decide: two calls of one size give the same bits, a window among more or
- * fewer images may differ in its float32 sum's last bits, and no result is off by more than 31 roundings of the sum of the magnitudes that
- * are added.  (rcv_i8_matmul: 4, and a row has the same bits whatever the other sizes.)  ReLU keeps a NaN.
+ * each step rounded, and infinite where it leaves the range: the sum's conversion (whole numbers above 2^24), its token scale, the weight
+ * scale and the bias in one step, the residual; the result is then rounded to out_dtype.  rcv_i8_conv3x3 converts and scales the sum of a
+ * tap, or of a run of a tap's channels, and adds these in float32 in an order that the sizes alone decide: two calls of one size give the
+ * same bits, a window among more or fewer images may differ in its float32 sum's last bits, and no result is off by more than 31
+ * roundings of the sum of the magnitudes that are added.  (rcv_i8_matmul: 4, and a row has the same bits whatever the other sizes.)  ReLU
+ * keeps a NaN.
  *   codes       rows codes_pitch bytes apart; 16-byte aligned, codes_pitch a multiple of 16, and the last row readable up to
  *               channels rounded up to a multiple of 16 (what lies there has no influence); -128 is allowed
  *   weights     [out_channels][taps][channels rounded up to a multiple of 128], 16-byte aligned, zeros behind `channels`
